@@ -12,6 +12,7 @@ LIB_PATH = os.path.join(PKG, "libagb_cuda.so")
 AGB_OK = 0
 AGB_F32, AGB_BF16, AGB_F64 = 0, 1, 2
 REDUCE_SUM, REDUCE_MEAN, REDUCE_MAX = 0, 1, 2
+AGB_I32, AGB_I64 = 0, 1
 
 # name -> (restype, argtypes); must list every symbol include/agb/agb.h declares
 _vp, _i64, _i, _f, _sz = C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_size_t
@@ -43,6 +44,12 @@ SIGNATURES = {
     "agb_layernorm_fwd": (_i, [_vp, _vp, _vp, _vp, _i64, _i64, _f, _i, _vp]),
     "agb_layernorm_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f, _i, _vp]),
     "agb_layernorm_jvp": (_i, [_vp, _vp, _vp, _vp, _i64, _i64, _f, _i, _vp]),
+    "agb_layernorm_affine_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f, _i, _vp]),
+    "agb_layernorm_affine_bwd_workspace_bytes": (_sz, [_i64, _i64, _i]),
+    "agb_layernorm_affine_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _sz, _i64, _i64, _i, _vp]),
+    "agb_distill_topk_fwd": (_i, [_vp, _vp, _i, _vp, _i, _vp, _vp, _i64, _i64, _i64, _f, _i, _vp]),
+    "agb_distill_topk_bwd": (_i, [_vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _f, _i, _vp]),
+    "agb_distill_topk_fwd_bwd": (_i, [_vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _f, _i, _vp]),
     "agb_softmax_row_fwd": (_i, [_vp, _vp, _i64, _i64, _i, _vp]),
     "agb_logsumexp_row_fwd": (_i, [_vp, _vp, _i64, _i64, _i, _vp]),
     "agb_softmax_row_bwd": (_i, [_vp, _vp, _vp, _vp, _i64, _i64, _i, _vp]),

@@ -1,6 +1,8 @@
 // agb_cuda.cu -- the C ABI of libagb_cuda.so (declared in include/agb/agb.h) and the launch
-// heuristics behind it.  Single translation unit: all kernels are included here.
+// heuristics behind it.  The kernels of the norm and softmax families are included here; the operators at the end of
+// a model (LayerNorm with weight and bias, vocabulary loss, distillation loss) are in agb_train.cu.
 #include "agb/agb.h"
+#include "agb_internal.h"
 
 #include <nvtx3/nvToolsExt.h>
 
@@ -1549,3 +1551,40 @@ int agb_reduce_all(int op, const void* x, void* out, int64_t n, int dtype, void*
 #include "agb_shard.cuh"
 #include "agb_peer.cuh"
 #include "agb_host.cuh"
+
+// ====================================================================== shared with the other translation unit
+namespace agb_int {
+
+int fail(int code, const char* fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(t_err, sizeof(t_err), fmt, ap);
+    va_end(ap);
+    return code;
+}
+int cuda_fail(cudaError_t e, const char* what) { return ::cuda_fail(e, what); }
+int after_launch(const char* what) { return ::after_launch(what); }
+int check_ptr(const void* p, const char* name, int elem, bool required) { return ::check_ptr(p, name, elem, required); }
+
+int device(Device* out) {
+    const DevInfo* d;
+    AGB_TRY(device_info(&d));
+    int dev = 0;
+    AGB_CUDA(cudaGetDevice(&dev));
+    static std::mutex mu;
+    static int* status[kMaxDevices] = {};
+    std::lock_guard<std::mutex> lk(mu);
+    if (!status[dev]) {
+        void* p = nullptr;
+        AGB_CUDA(cudaGetSymbolAddress(&p, agb::g_device_status));
+        status[dev] = static_cast<int*>(p);
+    }
+    out->sms = d->sms;
+    out->smem_optin = d->smem_optin;
+    out->smem_per_sm = d->smem_per_sm;
+    out->status = status[dev];
+    return AGB_OK;
+}
+bool pdl_enabled() { return opt_pdl.load() != 0; }
+
+}  // namespace agb_int

@@ -10,9 +10,11 @@
 namespace agb {
 
 // Device-global status word: 0 = ok, otherwise an agb_status_t written by a kernel whose
-// bounded wait ran out.  Read and cleared by agb_device_status().
-// (defined here: the library is a single translation unit)
+// bounded wait ran out.  Read and cleared by agb_device_status().  It lives in agb_cuda.cu's translation unit; the
+// kernels of the other one are handed its address.
+#ifndef AGB_NO_STATUS_WORD
 __device__ int g_device_status = 0;
+#endif
 
 // A wait gives up after kWaitPollLimit polls of mbarrier.try_wait, each of which may suspend the
 // thread in hardware for up to kWaitSuspendNs: at most ~2.6 s in total.

@@ -216,6 +216,122 @@ def layernorm_jvp(y, t, var, eps=1e-5, out=None):
     return ty
 
 
+def _on(t):
+    """Makes t's device the current one (the library launches on the current device and its current stream)."""
+    return torch.cuda.device(t.device)
+
+
+def _out(t, shape, dtype, like, name):
+    """The caller's output tensor, checked, or a new one on like's device."""
+    if t is None:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != like.device or not t.is_contiguous():
+        raise ValueError(f"{name} {tuple(t.shape)} {t.dtype} on {t.device}: expected contiguous {tuple(shape)} {dtype} on {like.device}")
+    return t
+
+
+def _workspace(t, nbytes, like):
+    if t is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    if t.device != like.device or not t.is_contiguous():
+        raise ValueError(f"workspace on {t.device}: expected a contiguous tensor on {like.device}")
+    return t
+
+
+def layernorm_affine_fwd(x, gamma, beta=None, eps=1e-5, out=None, mean=None, rstd=None):
+    """y = (x - mean) * rstd * gamma + beta; returns (y, mean[rows], rstd[rows]), the statistics in fp32."""
+    rows, hidden = _rows_hidden(x)
+    with _on(x):
+        y = torch.empty_like(x) if out is None else out
+        mean, rstd = _out(mean, (rows,), torch.float32, x, "mean"), _out(rstd, (rows,), torch.float32, x, "rstd")
+        _same(x, y)
+        _vec(x, hidden, x.dtype, gamma, beta)
+        check(_lib.lib().agb_layernorm_affine_fwd(_p(x), _p(gamma), _p(beta), _p(y), _p(mean), _p(rstd), rows, hidden, eps, _dt(x),
+                                                  _stream()))
+    return y, mean, rstd
+
+
+def layernorm_affine_bwd(x, gamma, mean, rstd, gy, dx_add=None, dx=None, dgamma=None, dbeta=None, accumulate=False, with_beta=True,
+                         workspace=None):
+    """Returns (dx, dgamma, dbeta): dgamma and dbeta fp32 [hidden], dbeta None without a bias (with_beta=False).  dx_add is added
+    to dx (may be gy or dx itself); with accumulate the column sums are added to the given dgamma and dbeta."""
+    rows, hidden = _rows_hidden(x)
+    if accumulate and (dgamma is None or (with_beta and dbeta is None)):
+        raise ValueError("accumulate needs the tensors to add to")
+    if dbeta is not None and not with_beta:
+        raise ValueError("dbeta given with with_beta=False")
+    with _on(x):
+        dx = torch.empty_like(x) if dx is None else dx
+        dgamma = _out(dgamma, (hidden,), torch.float32, x, "dgamma")
+        dbeta = _out(dbeta, (hidden,), torch.float32, x, "dbeta") if with_beta else None
+        _same(x, gy, dx_add, dx)
+        _vec(x, hidden, x.dtype, gamma)
+        _vec(x, rows, torch.float32, mean, rstd)
+        ws = _workspace(workspace, _lib.lib().agb_layernorm_affine_bwd_workspace_bytes(rows, hidden, _dt(x)), x)
+        check(_lib.lib().agb_layernorm_affine_bwd(_p(x), _p(gamma), _p(mean), _p(rstd), _p(gy), _p(dx_add), _p(dx), _p(dgamma), _p(dbeta),
+                                                  int(bool(accumulate)), _p(ws), ws.numel() * ws.element_size(), rows, hidden, _dt(x),
+                                                  _stream()))
+    return dx, dgamma, dbeta
+
+
+_IT = {torch.int32: _lib.AGB_I32, torch.int64: _lib.AGB_I64}
+
+
+def _it(t, name):
+    try:
+        return _IT[t.dtype]
+    except KeyError:
+        raise TypeError(f"{name}: unsupported index dtype {t.dtype}: int32 or int64 only") from None
+
+
+def _distill_operands(z, idx, teacher):
+    rows, vocab = _rows_hidden(z)
+    k = idx.shape[-1] if idx.dim() else 0
+    if k <= 0 or tuple(idx.shape) != tuple(z.shape[:-1]) + (k,) or tuple(teacher.shape) != tuple(idx.shape):
+        raise ValueError(f"idx {tuple(idx.shape)} and teacher {tuple(teacher.shape)} must both be {tuple(z.shape[:-1])} + (k,)")
+    for t, name in ((idx, "idx"), (teacher, "teacher")):
+        if t.device != z.device or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous on {z.device}")
+    return rows, vocab, k
+
+
+def distill_topk_fwd(z, idx, teacher, temperature=1.0, loss=None, lse=None):
+    """Loss of the student's logits z [.., vocab] against the teacher's logits teacher [.., k] at the columns idx [.., k]:
+    temperature^2 * KL(softmax_k(teacher / t) || softmax(z / t)); returns (loss[rows], lse[rows]) in fp32.  Entries whose index
+    lies outside [0, vocab) take no part; a row without entries has loss = lse = 0."""
+    rows, vocab, k = _distill_operands(z, idx, teacher)
+    with _on(z):
+        loss, lse = _out(loss, (rows,), torch.float32, z, "loss"), _out(lse, (rows,), torch.float32, z, "lse")
+        check(_lib.lib().agb_distill_topk_fwd(_p(z), _p(idx), _it(idx, "idx"), _p(teacher), _dt(teacher), _p(loss), _p(lse), rows, vocab,
+                                              k, temperature, _dt(z), _stream()))
+    return loss, lse
+
+
+def distill_topk_bwd(z, idx, teacher, lse, gy, temperature=1.0, dz_add=None, dz=None):
+    """dz = gy[rows] * t * (softmax(z / t) - the teacher's shares) [+ dz_add], lse from distill_topk_fwd."""
+    rows, vocab, k = _distill_operands(z, idx, teacher)
+    with _on(z):
+        dz = torch.empty_like(z) if dz is None else dz
+        _same(z, dz_add, dz)
+        _vec(z, rows, torch.float32, lse, gy)
+        check(_lib.lib().agb_distill_topk_bwd(_p(z), _p(idx), _it(idx, "idx"), _p(teacher), _dt(teacher), _p(lse), _p(gy), _p(dz_add),
+                                              _p(dz), rows, vocab, k, temperature, _dt(z), _stream()))
+    return dz
+
+
+def distill_topk_fwd_bwd(z, idx, teacher, gy, temperature=1.0, dz_add=None, loss=None, lse=None, dz=None):
+    """Both in one pass over the logits, for a gy known beforehand; returns (loss, lse, dz).  dz may be z itself."""
+    rows, vocab, k = _distill_operands(z, idx, teacher)
+    with _on(z):
+        loss, lse = _out(loss, (rows,), torch.float32, z, "loss"), _out(lse, (rows,), torch.float32, z, "lse")
+        dz = torch.empty_like(z) if dz is None else dz
+        _same(z, dz_add, dz)
+        _vec(z, rows, torch.float32, gy)
+        check(_lib.lib().agb_distill_topk_fwd_bwd(_p(z), _p(idx), _it(idx, "idx"), _p(teacher), _dt(teacher), _p(gy), _p(dz_add), _p(loss),
+                                                  _p(lse), _p(dz), rows, vocab, k, temperature, _dt(z), _stream()))
+    return loss, lse, dz
+
+
 def softmax_row(z, out=None):
     """cgadimpl's softmax_row: softmax over the last axis."""
     rows, hidden = _rows_hidden(z)

@@ -52,6 +52,7 @@ typedef enum {
 
 typedef enum { AGB_F32 = 0, AGB_BF16 = 1, AGB_F64 = 2 } agb_dtype_t;
 typedef enum { AGB_REDUCE_SUM = 0, AGB_REDUCE_MEAN = 1, AGB_REDUCE_MAX = 2 } agb_reduce_op_t;
+typedef enum { AGB_I32 = 0, AGB_I64 = 1 } agb_index_t;   /* type of index arrays (targets, teacher columns) */
 
 typedef void* agb_stream_t; /* cudaStream_t */
 
@@ -244,6 +245,45 @@ int agb_layernorm_bwd(const void* x, const float* mean, const float* var, const 
  *   tmean = mean_j t;  d = mean_j y*(t - tmean);  ty = (1/sqrt(var+eps)) * ((t - tmean) - y*d). */
 int agb_layernorm_jvp(const void* y, const void* t, const float* var, void* ty, int64_t rows, int64_t hidden, float eps,
                       int dtype, agb_stream_t stream);
+
+/* ---- LayerNorm with weight and bias ----
+ * The reference's laynor has neither.  x, y, gy, dx, gamma, beta in `dtype`; mean, rstd [rows], dgamma, dbeta [hidden]
+ * in fp32 (so a 16-bit weight gets its gradient unrounded, as dgamma of the RMSNorm does).
+ *   mean = mean_j x;  rstd = 1 / sqrt(mean_j (x - mean)^2 + eps);  xh = (x - mean) * rstd
+ *   y  = xh * gamma + beta                                    (beta == NULL: no bias)
+ *   v  = gy * gamma;  dx = rstd * (v - mean_j v - xh * mean_j(v * xh))   [+ dx_add]
+ *   dgamma[j] = sum_r gy * xh;  dbeta[j] = sum_r gy           (either may be NULL; added to the old contents with
+ *                                                              `accumulate`; rows == 0 gives zeros, or leaves them)
+ * dx_add may alias gy or dx.  Sums in fp32, over the CTAs in fp64 in a fixed order: the same call gives the same bits.
+ * The workspace is only needed for dgamma or dbeta. */
+int agb_layernorm_affine_fwd(const void* x, const void* gamma, const void* beta, void* y, float* mean, float* rstd,
+                             int64_t rows, int64_t hidden, float eps, int dtype, agb_stream_t stream);
+size_t agb_layernorm_affine_bwd_workspace_bytes(int64_t rows, int64_t hidden, int dtype);
+int agb_layernorm_affine_bwd(const void* x, const void* gamma, const float* mean, const float* rstd, const void* gy,
+                             const void* dx_add, void* dx, float* dgamma, float* dbeta, int accumulate,
+                             void* workspace, size_t workspace_bytes, int64_t rows, int64_t hidden, int dtype,
+                             agb_stream_t stream);
+
+/* ---- distillation from a teacher's K largest logits ----
+ * The reference registers kldivergence without building it.  z [rows, vocab] student logits; idx [rows, k] columns
+ * (`idx_type`), teacher [rows, k] the teacher's logits there (`teacher_dtype`, AGB_F32 or AGB_BF16); k <= 1024.
+ *   p = softmax_k(teacher / t);  q = softmax_j(z / t);  lse = log sum_j exp(z / t)       (t: the temperature)
+ *   loss[r] = t^2 * sum_k p_k * (log p_k - log q[idx_k])
+ *   dz[r,j] = gy[r] * t * (q_j - sum of p_k over the k with idx_k = j)   [+ dz_add]
+ * An entry whose index lies outside [0, vocab) or whose teacher logit is -inf takes no part; a column named twice gets
+ * both shares.  A row without entries has no loss and no gradient, whatever its logits hold: loss = lse = 0, dz = 0
+ * (or dz_add).  loss, lse, gy: fp32 [rows].  dz may alias z, dz_add may alias dz.
+ * _fwd writes loss and lse, _bwd reads lse, _fwd_bwd does both for callers that know gy beforehand (a sum or a mean) and
+ * reads the logits from memory once. */
+int agb_distill_topk_fwd(const void* z, const void* idx, int idx_type, const void* teacher, int teacher_dtype,
+                         float* loss, float* lse, int64_t rows, int64_t vocab, int64_t k, float temperature,
+                         int dtype, agb_stream_t stream);
+int agb_distill_topk_bwd(const void* z, const void* idx, int idx_type, const void* teacher, int teacher_dtype,
+                         const float* lse, const float* gy, const void* dz_add, void* dz,
+                         int64_t rows, int64_t vocab, int64_t k, float temperature, int dtype, agb_stream_t stream);
+int agb_distill_topk_fwd_bwd(const void* z, const void* idx, int idx_type, const void* teacher, int teacher_dtype,
+                             const float* gy, const void* dz_add, float* loss, float* lse, void* dz,
+                             int64_t rows, int64_t vocab, int64_t k, float temperature, int dtype, agb_stream_t stream);
 
 /* ---- row softmax / logsumexp over the last axis and their rules ----
  * agb_softmax_row_fwd replaces softmax_row_nodeops (cgadimpl/src/ops/reduction.cpp:42-53):
