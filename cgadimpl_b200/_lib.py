@@ -47,6 +47,9 @@ SIGNATURES = {
     "agb_layernorm_affine_fwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f, _i, _vp]),
     "agb_layernorm_affine_bwd_workspace_bytes": (_sz, [_i64, _i64, _i]),
     "agb_layernorm_affine_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _sz, _i64, _i64, _i, _vp]),
+    "agb_linear_ce_workspace_bytes": (_sz, [_i, _i64, _i64, _i64, _i]),
+    "agb_linear_ce_fwd": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _i64, _i64, _i64, _i, _vp, _sz, _vp]),
+    "agb_linear_ce_bwd": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i64, _i64, _i64, _i, _vp, _sz, _vp]),
     "agb_distill_topk_fwd": (_i, [_vp, _vp, _i, _vp, _i, _vp, _vp, _i64, _i64, _i64, _f, _i, _vp]),
     "agb_distill_topk_bwd": (_i, [_vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _f, _i, _vp]),
     "agb_distill_topk_fwd_bwd": (_i, [_vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _f, _i, _vp]),

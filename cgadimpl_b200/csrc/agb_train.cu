@@ -7,6 +7,7 @@
 #include "agb_internal.h"
 #include "distill_topk.cuh"
 #include "layernorm_affine.cuh"
+#include "linear_ce.cuh"
 
 namespace {
 
@@ -175,9 +176,357 @@ int run_kd(const void* z, const void* idx, int idx_type, const void* teacher, in
     return dtype == AGB_F32 ? launch_kd<float, MODE>(a, rows, st) : launch_kd<bf16, MODE>(a, rows, st);
 }
 
+// ------------------------------------------------------------------ cross entropy from the hidden states
+// The driver's tensor map encoder, looked up once (the runtime library is linked, the driver library is not).
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+    static const EncodeTiled f = []() -> EncodeTiled {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            return nullptr;
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return f;
+}
+// A [planes][rows][cols] bf16 tensor with rows `stride` elements apart, read in boxes of 64 columns by `box_rows` rows.
+int make_map(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int planes, int64_t stride, int64_t plane, int box_rows) {
+    EncodeTiled f = encode_tiled();
+    if (!f) return fail(AGB_ERR_CUDA, "cuTensorMapEncodeTiled is not available in this driver");
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(planes)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(stride) * 2, static_cast<cuuint64_t>(plane) * 2};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_rows), 1};
+    const cuuint32_t steps[3] = {1, 1, 1};
+    const CUresult r = f(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, steps,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(AGB_ERR_CUDA, "cuTensorMapEncodeTiled: error %d", static_cast<int>(r));
+    return AGB_OK;
+}
+
+constexpr int64_t kCePackLimit = 512LL << 20;   // bytes of W laid out at once, where it has to be
+constexpr int64_t kCeGLimit = 256LL << 20;      // bytes of g at once
+
+// How a call is cut up, and where its parts lie in the workspace.
+struct CePlan {
+    int planes;
+    bool direct_w;              // TMA reads W as it is
+    int64_t rows_pad, k_stride, piece, pieces, g_stride, dh_stride, pairs;
+    int splits, k_per_split;
+    size_t h, w, count, row_of, pos_of, target_of, lse_of, gy_of, z_target, pair_at, g, dh, total;
+};
+
+CePlan plan_ce(bool backward, int64_t rows, int64_t hidden, int64_t vocab, int dtype, bool want_dh, int sms) {
+    CePlan p{};
+    p.planes = dtype == AGB_F32 ? 3 : 1;
+    p.direct_w = dtype == AGB_BF16 && hidden % 8 == 0;
+    p.rows_pad = ceil_div(rows, agb::kTM) * agb::kTM;
+    p.k_stride = ceil_div(hidden, 8) * 8;
+    p.piece = ceil_div(vocab, 256) * 256;
+    auto limit = [&](int64_t bytes_per_column, int64_t bytes) {
+        int64_t most = bytes / bytes_per_column / 256 * 256;
+        if (most < 256) most = 256;
+        if (p.piece > most) p.piece = most;
+    };
+    if (!p.direct_w) limit(p.planes * p.k_stride * 2, kCePackLimit);
+    if (backward) limit(p.planes * p.rows_pad * 2, kCeGLimit);
+    p.pieces = ceil_div(vocab, p.piece);
+    p.piece = ceil_div(ceil_div(vocab, p.pieces), 256) * 256;      // even pieces
+    p.pieces = ceil_div(vocab, p.piece);
+    p.g_stride = p.piece;
+    p.dh_stride = ceil_div(hidden, 4) * 4;
+    p.pairs = p.pieces * (p.piece / 128);
+    // dh: few tiles with a long sum are cut along it, until the GPU has two per SM or a part has 16 slabs
+    const int64_t tiles = p.rows_pad / agb::kTM * ceil_div(hidden, agb::kTN), blocks = ceil_div(p.piece, agb::kTK);
+    int64_t s = ceil_div(2 * sms, tiles);
+    if (s > blocks / 16) s = blocks / 16;
+    if (s < 1) s = 1;
+    p.k_per_split = static_cast<int>(ceil_div(blocks, s) * agb::kTK);
+    p.splits = static_cast<int>(ceil_div(p.piece, p.k_per_split));
+    size_t at = 0;
+    auto take = [&](size_t* where, size_t bytes) {
+        *where = at;
+        at += (bytes + 1023) / 1024 * 1024;
+    };
+    take(&p.h, static_cast<size_t>(p.planes) * p.rows_pad * p.k_stride * 2);
+    take(&p.count, 4);
+    take(&p.row_of, p.rows_pad * 4);
+    take(&p.pos_of, p.rows_pad * 4);
+    take(&p.target_of, p.rows_pad * 4);
+    if (!p.direct_w) take(&p.w, static_cast<size_t>(p.planes) * p.piece * p.k_stride * 2);
+    if (backward) {
+        take(&p.lse_of, p.rows_pad * 4);
+        take(&p.gy_of, p.rows_pad * 4);
+        take(&p.g, static_cast<size_t>(p.planes) * p.rows_pad * p.g_stride * 2);
+        if (want_dh) take(&p.dh, static_cast<size_t>(p.splits) * p.rows_pad * p.dh_stride * 4);
+    } else {
+        take(&p.z_target, p.rows_pad * 4);
+        take(&p.pair_at, static_cast<size_t>(p.pairs) * p.rows_pad * 8);
+    }
+    p.total = at + 1024;        // the caller's base may lie anywhere
+    return p;
+}
+
+int check_ce(int64_t rows, int64_t hidden, int64_t vocab, int dtype, int target_type) {
+    if (rows < 0 || hidden <= 0 || vocab <= 0)
+        return fail(AGB_ERR_INVALID_ARG, "rows=%lld hidden=%lld vocab=%lld", (long long)rows, (long long)hidden, (long long)vocab);
+    if (dtype != AGB_F32 && dtype != AGB_BF16) return fail(AGB_ERR_UNSUPPORTED, "dtype %d (only AGB_F32, AGB_BF16)", dtype);
+    if (target_type != AGB_I32 && target_type != AGB_I64) return fail(AGB_ERR_INVALID_ARG, "target_type %d (AGB_I32 or AGB_I64)", target_type);
+    if (rows > (1LL << 24) || hidden > (1LL << 20) || vocab > (1LL << 24))
+        return fail(AGB_ERR_UNSUPPORTED, "rows=%lld hidden=%lld vocab=%lld (at most 2^24, 2^20, 2^24)", (long long)rows, (long long)hidden,
+                    (long long)vocab);
+    return AGB_OK;
+}
+
+struct CeCall {
+    const void *h, *w, *target;
+    int target_type;
+    int64_t rows, hidden, vocab;
+    int dtype;
+    char* ws;
+    cudaStream_t st;
+    agb_int::Device d;
+    CePlan p;
+    template <typename T>
+    T* at(size_t off) const { return reinterpret_cast<T*>(ws + off); }
+};
+
+int ce_rows(const CeCall& c, const float* lse, const float* gy, float* loss, float* lse_out) {
+    agb::CeRowsArgs a{};
+    a.x = c.h;
+    a.target = c.target;
+    a.target64 = c.target_type == AGB_I64;
+    a.rows = c.rows;
+    a.cols = static_cast<int>(c.hidden);
+    a.vocab = static_cast<int>(c.vocab);
+    a.planes = c.p.planes;
+    a.dst = c.at<bf16>(c.p.h);
+    a.rows_pad = c.p.rows_pad;
+    a.stride = c.p.k_stride;
+    a.count = c.at<int>(c.p.count);
+    a.row_of = c.at<int>(c.p.row_of);
+    a.pos_of = c.at<int>(c.p.pos_of);
+    a.target_of = c.at<int>(c.p.target_of);
+    a.lse = lse;
+    a.gy = gy;
+    if (lse) {
+        a.lse_of = c.at<float>(c.p.lse_of);
+        a.gy_of = c.at<float>(c.p.gy_of);
+    }
+    a.loss = loss;
+    a.lse_out = lse_out;
+    const unsigned grid = static_cast<unsigned>(ceil_div(c.rows, agb::kRowsBlock));
+    if (c.dtype == AGB_F32) agb::ce_rows_kernel<float><<<grid, 256, 0, c.st>>>(a);
+    else agb::ce_rows_kernel<bf16><<<grid, 256, 0, c.st>>>(a);
+    return after_launch("linear_ce_rows");
+}
+int ce_pack(const CeCall& c, int64_t col0, int64_t n) {
+    if (c.p.direct_w) return AGB_OK;
+    int64_t grid = ceil_div(n, 8);
+    if (grid > 16LL * c.d.sms) grid = 16LL * c.d.sms;
+    if (c.dtype == AGB_F32)
+        agb::ce_pack_kernel<float><<<static_cast<unsigned>(grid), 256, 0, c.st>>>(static_cast<const float*>(c.w) + col0 * c.hidden, n, (int)c.hidden,
+                                                                                 c.at<bf16>(c.p.w), c.p.piece, c.p.k_stride);
+    else
+        agb::ce_pack_kernel<bf16><<<static_cast<unsigned>(grid), 256, 0, c.st>>>(static_cast<const bf16*>(c.w) + col0 * c.hidden, n, (int)c.hidden,
+                                                                                c.at<bf16>(c.p.w), c.p.piece, c.p.k_stride);
+    return after_launch("linear_ce_pack");
+}
+// W, or its piece where it was laid out: rows of the map, and the map's row of the piece's first column.
+int map_w(const CeCall& c, CUtensorMap* m, int64_t n, int box_rows) {
+    if (c.p.direct_w) return make_map(m, c.w, c.hidden, c.vocab, 1, c.hidden, c.vocab * c.hidden, box_rows);
+    return make_map(m, c.at<void>(c.p.w), c.p.k_stride, n, c.p.planes, c.p.k_stride, c.p.piece * c.p.k_stride, box_rows);
+}
+int map_h(const CeCall& c, CUtensorMap* m, int box_rows) {
+    return make_map(m, c.at<void>(c.p.h), c.p.k_stride, c.p.rows_pad, c.p.planes, c.p.k_stride, c.p.rows_pad * c.p.k_stride, box_rows);
+}
+int map_g(const CeCall& c, CUtensorMap* m, int box_rows) {
+    return make_map(m, c.at<void>(c.p.g), c.p.g_stride, c.p.rows_pad, c.p.planes, c.p.g_stride, c.p.rows_pad * c.p.g_stride, box_rows);
+}
+agb::CeArgs ce_args(const CeCall& c) {
+    agb::CeArgs a{};
+    a.count = c.at<int>(c.p.count);
+    a.status = c.d.status;
+    a.rows_pad = c.p.rows_pad;
+    a.target = c.at<int>(c.p.target_of);
+    a.vocab = static_cast<int>(c.vocab);
+    a.planes = c.p.planes;
+    a.hidden = static_cast<int>(c.hidden);
+    return a;
+}
+// The logits of a piece: rows that take part x n columns.
+agb::CeJob logits_job(const CeCall& c, int epi, int64_t col0, int64_t n) {
+    agb::CeJob j{};
+    j.epi = epi;
+    j.a_planes3 = c.p.planes == 3;
+    j.b_row0 = c.p.direct_w ? static_cast<int>(col0) : 0;
+    j.m = -1;
+    j.n = static_cast<int>(n);
+    j.k = static_cast<int>(c.hidden);
+    j.splits = 1;
+    j.k_per_split = static_cast<int>(ceil_div(c.hidden, agb::kTK) * agb::kTK);
+    return j;
+}
+int launch_gemm(const CeCall& c, const agb::CeArgs& a) {
+    int64_t tiles = 0;
+    for (int i = 0; i < a.jobs; ++i) {
+        const agb::CeJob& j = a.job[i];
+        tiles += ceil_div(j.m < 0 ? c.rows : j.m, agb::kTM) * ceil_div(j.n, agb::kTN) * j.splits;
+    }
+    if (tiles >= (1LL << 31)) return fail(AGB_ERR_UNSUPPORTED, "too many tiles");
+    AGB_CUDA(cudaFuncSetAttribute(agb::ce_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, agb::kCeSmem));
+    const unsigned grid = static_cast<unsigned>(tiles < c.d.sms ? tiles : c.d.sms);
+    agb::ce_gemm_kernel<<<grid, agb::kCeThreads, agb::kCeSmem, c.st>>>(a);
+    return after_launch("linear_ce_gemm");
+}
+
+int start_ce(CeCall* c, bool backward, bool want_dh, void* workspace, size_t workspace_bytes, agb_stream_t stream) {
+    const int elem = c->dtype == AGB_F32 ? 4 : 2;
+    AGB_TRY(check_ptr(c->h, "h", elem));
+    AGB_TRY(check_ptr(c->w, "w", elem));
+    AGB_TRY(check_ptr(c->target, "target", c->target_type == AGB_I64 ? 8 : 4));
+    if (c->dtype == AGB_BF16 && c->hidden % 8 == 0 && addr(c->w) % 16)
+        return fail(AGB_ERR_MISALIGNED, "w must be aligned to 16 bytes where hidden is a multiple of 8");
+    if (!workspace) return fail(AGB_ERR_WORKSPACE, "workspace is NULL");
+    AGB_TRY(agb_int::device(&c->d));
+    c->p = plan_ce(backward, c->rows, c->hidden, c->vocab, c->dtype, want_dh, c->d.sms);
+    if (workspace_bytes < c->p.total) return fail(AGB_ERR_WORKSPACE, "workspace %zu bytes, need %zu", workspace_bytes, c->p.total);
+    c->ws = reinterpret_cast<char*>((addr(workspace) + 1023) & ~static_cast<uintptr_t>(1023));
+    c->st = static_cast<cudaStream_t>(stream);
+    return AGB_OK;
+}
+
 }  // namespace
 
 extern "C" {
+
+size_t agb_linear_ce_workspace_bytes(int backward, int64_t rows, int64_t hidden, int64_t vocab, int dtype) {
+    agb_int::Device d;
+    if (check_ce(rows, hidden, vocab, dtype, AGB_I32) != AGB_OK || agb_int::device(&d) != AGB_OK) return 0;
+    return plan_ce(backward != 0, rows > 0 ? rows : 1, hidden, vocab, dtype, true, d.sms).total;
+}
+
+int agb_linear_ce_fwd(const void* h, const void* w, const void* target, int target_type, float* loss, float* lse, int64_t rows,
+                      int64_t hidden, int64_t vocab, int dtype, void* workspace, size_t workspace_bytes, agb_stream_t stream) {
+    AGB_RANGE();
+    AGB_TRY(check_ce(rows, hidden, vocab, dtype, target_type));
+    if (rows == 0) return AGB_OK;
+    AGB_TRY(check_ptr(loss, "loss", 4));
+    AGB_TRY(check_ptr(lse, "lse", 4));
+    CeCall c{h, w, target, target_type, rows, hidden, vocab, dtype, nullptr, nullptr, {}, {}};
+    AGB_TRY(start_ce(&c, false, false, workspace, workspace_bytes, stream));
+    AGB_TRY(ce_rows(c, nullptr, nullptr, loss, lse));
+    for (int64_t i = 0; i < c.p.pieces; ++i) {
+        const int64_t col0 = i * c.p.piece, n = vocab - col0 < c.p.piece ? vocab - col0 : c.p.piece;
+        AGB_TRY(ce_pack(c, col0, n));
+        agb::CeArgs a = ce_args(c);
+        AGB_TRY(map_h(c, &a.A[0], 128));
+        AGB_TRY(map_w(c, &a.B[0], n, 128));
+        a.jobs = 1;
+        a.job[0] = logits_job(c, agb::kEpiPairs, col0, n);
+        a.pairs = c.at<float2>(c.p.pair_at);
+        a.z_target = c.at<float>(c.p.z_target);
+        a.col0 = static_cast<int>(col0);
+        a.pair0 = static_cast<int>(col0 / 128);
+        AGB_TRY(launch_gemm(c, a));
+    }
+    const int64_t last = vocab - (c.p.pieces - 1) * c.p.piece;
+    const int pairs = static_cast<int>((c.p.pieces - 1) * (c.p.piece / 128) + ceil_div(last, agb::kTN) * 2);
+    agb::ce_join_kernel<<<static_cast<unsigned>(ceil_div(rows, 32)), dim3(32, 8), 0, c.st>>>(
+        c.at<float2>(c.p.pair_at), pairs, c.p.rows_pad, c.at<int>(c.p.count), c.at<float>(c.p.z_target), c.at<int>(c.p.row_of), loss, lse);
+    return after_launch("linear_ce_join");
+}
+
+int agb_linear_ce_bwd(const void* h, const void* w, const void* target, int target_type, const float* lse, const float* gy, void* dh,
+                      void* dw, int accumulate_dw, int64_t rows, int64_t hidden, int64_t vocab, int dtype, void* workspace,
+                      size_t workspace_bytes, agb_stream_t stream) {
+    AGB_RANGE();
+    AGB_TRY(check_ce(rows, hidden, vocab, dtype, target_type));
+    const int elem = dtype == AGB_F32 ? 4 : 2;
+    if (!dh && !dw) return fail(AGB_ERR_INVALID_ARG, "neither dh nor dw is asked for");
+    AGB_TRY(check_ptr(dw, "dw", elem, false));
+    if (rows == 0) {
+        if (dw && !accumulate_dw)
+            AGB_CUDA(cudaMemsetAsync(dw, 0, static_cast<size_t>(vocab) * hidden * elem, static_cast<cudaStream_t>(stream)));
+        return AGB_OK;
+    }
+    AGB_TRY(check_ptr(dh, "dh", elem, false));
+    AGB_TRY(check_ptr(lse, "lse", 4));
+    AGB_TRY(check_ptr(gy, "gy", 4));
+    CeCall c{h, w, target, target_type, rows, hidden, vocab, dtype, nullptr, nullptr, {}, {}};
+    AGB_TRY(start_ce(&c, true, dh != nullptr, workspace, workspace_bytes, stream));
+    AGB_TRY(ce_rows(c, lse, gy, nullptr, nullptr));
+    for (int64_t i = 0; i < c.p.pieces; ++i) {
+        const int64_t col0 = i * c.p.piece, n = vocab - col0 < c.p.piece ? vocab - col0 : c.p.piece;
+        AGB_TRY(ce_pack(c, col0, n));
+        agb::CeArgs a = ce_args(c);
+        AGB_TRY(map_h(c, &a.A[0], 128));
+        AGB_TRY(map_w(c, &a.B[0], n, 128));
+        a.jobs = 1;
+        a.job[0] = logits_job(c, agb::kEpiG, col0, n);
+        a.col0 = static_cast<int>(col0);
+        a.lse = c.at<float>(c.p.lse_of);
+        a.gy = c.at<float>(c.p.gy_of);
+        a.g = c.at<bf16>(c.p.g);
+        a.g_stride = c.p.g_stride;
+        AGB_TRY(launch_gemm(c, a));
+        a.jobs = 0;
+        if (dh) {
+            agb::CeJob& j = a.job[a.jobs];
+            j = agb::CeJob{};
+            j.epi = agb::kEpiDh;
+            j.b_mn = 1;
+            j.a_planes3 = c.p.planes == 3;
+            j.b_row0 = c.p.direct_w ? static_cast<int>(col0) : 0;
+            j.m = -1;
+            j.n = static_cast<int>(hidden);
+            j.k = static_cast<int>(n);
+            j.splits = c.p.splits;
+            j.k_per_split = c.p.k_per_split;
+            j.n_first = 1;
+            AGB_TRY(map_g(c, &a.A[a.jobs], 128));
+            AGB_TRY(map_w(c, &a.B[a.jobs], n, 64));
+            a.dh = c.at<float>(c.p.dh);
+            a.dh_stride = c.p.dh_stride;
+            a.dh_add = i > 0;
+            ++a.jobs;
+        }
+        if (dw) {
+            agb::CeJob& j = a.job[a.jobs];
+            j = agb::CeJob{};
+            j.epi = agb::kEpiDw;
+            j.a_mn = j.b_mn = 1;
+            j.a_planes3 = c.p.planes == 3;
+            j.m = static_cast<int>(n);
+            j.n = static_cast<int>(hidden);
+            j.k = -1;
+            j.splits = 1;
+            j.k_per_split = static_cast<int>(c.p.rows_pad);
+            j.n_first = 1;
+            AGB_TRY(map_g(c, &a.A[a.jobs], 64));
+            AGB_TRY(map_h(c, &a.B[a.jobs], 64));
+            a.dw = dw;
+            a.dw_add = accumulate_dw != 0;
+            a.dw_f32 = dtype == AGB_F32;
+            ++a.jobs;
+        }
+        AGB_TRY(launch_gemm(c, a));
+    }
+    if (dh) {
+        const unsigned grid = static_cast<unsigned>(rows < 16LL * c.d.sms ? rows : 16LL * c.d.sms);
+        if (dtype == AGB_F32)
+            agb::ce_dh_kernel<float><<<grid, 256, 0, c.st>>>(c.at<float>(c.p.dh), c.p.splits, c.p.rows_pad, c.p.dh_stride, c.at<int>(c.p.pos_of),
+                                                             static_cast<float*>(dh), rows, (int)hidden);
+        else
+            agb::ce_dh_kernel<bf16><<<grid, 256, 0, c.st>>>(c.at<float>(c.p.dh), c.p.splits, c.p.rows_pad, c.p.dh_stride, c.at<int>(c.p.pos_of),
+                                                            static_cast<bf16*>(dh), rows, (int)hidden);
+        return after_launch("linear_ce_dh");
+    }
+    return AGB_OK;
+}
 
 int agb_layernorm_affine_fwd(const void* x, const void* gamma, const void* beta, void* y, float* mean, float* rstd, int64_t rows,
                              int64_t hidden, float eps, int dtype, agb_stream_t stream) {

@@ -284,6 +284,45 @@ def _it(t, name):
         raise TypeError(f"{name}: unsupported index dtype {t.dtype}: int32 or int64 only") from None
 
 
+def _ce_operands(h, w, target):
+    rows, hidden = _rows_hidden(h)
+    if w.dim() != 2 or w.shape[1] != hidden or w.shape[0] == 0 or w.dtype != h.dtype or w.device != h.device or not w.is_contiguous():
+        raise ValueError(f"w {tuple(w.shape)} {w.dtype} on {w.device}: expected contiguous [vocab, {hidden}] {h.dtype} on {h.device}")
+    if tuple(target.shape) != tuple(h.shape[:-1]) or target.device != h.device or not target.is_contiguous():
+        raise ValueError(f"target {tuple(target.shape)} on {target.device}: expected contiguous {tuple(h.shape[:-1])} on {h.device}")
+    return rows, hidden, w.shape[0]
+
+
+def linear_ce_fwd(h, w, target, loss=None, lse=None, workspace=None):
+    """Cross entropy of softmax(h w') against target (int32 or int64), the logits not kept; returns (loss[rows], lse[rows]) in fp32.
+    Rows whose target lies outside [0, vocab) take no part: loss = lse = 0."""
+    rows, hidden, vocab = _ce_operands(h, w, target)
+    with _on(h):
+        loss, lse = _out(loss, (rows,), torch.float32, h, "loss"), _out(lse, (rows,), torch.float32, h, "lse")
+        ws = _workspace(workspace, _lib.lib().agb_linear_ce_workspace_bytes(0, rows, hidden, vocab, _dt(h)), h)
+        check(_lib.lib().agb_linear_ce_fwd(_p(h), _p(w), _p(target), _it(target, "target"), _p(loss), _p(lse), rows, hidden, vocab, _dt(h),
+                                           _p(ws), ws.numel() * ws.element_size(), _stream()))
+    return loss, lse
+
+
+def linear_ce_bwd(h, w, target, lse, gy, dh=None, dw=None, accumulate_dw=False, need_dh=True, need_dw=True, workspace=None):
+    """Returns (dh, dw) for gy[rows], lse from linear_ce_fwd; need_dh / need_dw=False leaves one out (None)."""
+    rows, hidden, vocab = _ce_operands(h, w, target)
+    if accumulate_dw and dw is None:
+        raise ValueError("accumulate_dw needs the dw to add to")
+    with _on(h):
+        dh = (torch.empty_like(h) if dh is None else dh) if need_dh else None
+        dw = (torch.empty_like(w) if dw is None else dw) if need_dw else None
+        _same(h, dh)
+        _same(w, dw)
+        _vec(h, rows, torch.float32, lse, gy)
+        ws = _workspace(workspace, _lib.lib().agb_linear_ce_workspace_bytes(1, rows, hidden, vocab, _dt(h)), h)
+        check(_lib.lib().agb_linear_ce_bwd(_p(h), _p(w), _p(target), _it(target, "target"), _p(lse), _p(gy), _p(dh), _p(dw),
+                                           int(bool(accumulate_dw)), rows, hidden, vocab, _dt(h), _p(ws), ws.numel() * ws.element_size(),
+                                           _stream()))
+    return dh, dw
+
+
 def _distill_operands(z, idx, teacher):
     rows, vocab = _rows_hidden(z)
     k = idx.shape[-1] if idx.dim() else 0

@@ -264,6 +264,26 @@ int agb_layernorm_affine_bwd(const void* x, const void* gamma, const float* mean
                              void* workspace, size_t workspace_bytes, int64_t rows, int64_t hidden, int dtype,
                              agb_stream_t stream);
 
+/* ---- softmax cross entropy taken from the hidden states ----
+ * The reference registers linear and ce_with_logits without building them.  h [rows, hidden], w [vocab, hidden] in `dtype`,
+ * target [rows] (`target_type`); the logits z = h w' exist a piece at a time only.
+ *   lse[r] = log sum_v exp z[r,v];  loss[r] = lse[r] - z[r, target[r]]
+ *   g[r,v] = gy[r] * (exp(z[r,v] - lse[r]) - [v == target[r]]);  dh = g w;  dw = g' h   (added to the old dw with accumulate_dw)
+ * A row whose target lies outside [0, vocab) (-1, -100, ..) takes no part: loss = lse = 0, its dh is zero, and what its h
+ * holds reaches nothing.  loss, lse, gy: fp32 [rows].  dh or dw may be NULL.
+ * AGB_BF16: products of bf16 on the tensor cores with fp32 sums; g is rounded to bf16 as the operand of the two gradient
+ * products, dh and dw are rounded once.  AGB_F32: every operand as three bf16 planes and six products, fp32 accuracy.
+ * w is read by TMA: aligned to 16 bytes where hidden is a multiple of 8 (AGB_BF16).  Nothing is accumulated atomically: the same
+ * call gives the same bits.  The workspace (at most about 0.5 GB for w, 0.25 GB for g, plus the rows) need not be kept between the
+ * forward and the backward; agb_linear_ce_workspace_bytes needs a device (0 without one). */
+size_t agb_linear_ce_workspace_bytes(int backward, int64_t rows, int64_t hidden, int64_t vocab, int dtype);
+int agb_linear_ce_fwd(const void* h, const void* w, const void* target, int target_type, float* loss, float* lse,
+                      int64_t rows, int64_t hidden, int64_t vocab, int dtype, void* workspace, size_t workspace_bytes,
+                      agb_stream_t stream);
+int agb_linear_ce_bwd(const void* h, const void* w, const void* target, int target_type, const float* lse, const float* gy,
+                      void* dh, void* dw, int accumulate_dw, int64_t rows, int64_t hidden, int64_t vocab, int dtype,
+                      void* workspace, size_t workspace_bytes, agb_stream_t stream);
+
 /* ---- distillation from a teacher's K largest logits ----
  * The reference registers kldivergence without building it.  z [rows, vocab] student logits; idx [rows, k] columns
  * (`idx_type`), teacher [rows, k] the teacher's logits there (`teacher_dtype`, AGB_F32 or AGB_BF16); k <= 1024.
