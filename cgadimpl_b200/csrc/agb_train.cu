@@ -215,6 +215,7 @@ struct CePlan {
     int planes;
     bool direct_w;              // TMA reads W as it is
     int64_t rows_pad, k_stride, piece, pieces, g_stride, dh_stride, pairs;
+    int tn;                     // columns of a tile of logits
     int splits, k_per_split;
     size_t h, w, count, row_of, pos_of, target_of, lse_of, gy_of, z_target, pair_at, g, dh, total;
 };
@@ -223,7 +224,7 @@ CePlan plan_ce(bool backward, int64_t rows, int64_t hidden, int64_t vocab, int d
     CePlan p{};
     p.planes = dtype == AGB_F32 ? 3 : 1;
     p.direct_w = dtype == AGB_BF16 && hidden % 8 == 0;
-    p.rows_pad = ceil_div(rows, agb::kTM) * agb::kTM;
+    p.rows_pad = ceil_div(rows, 2 * agb::kTM) * 2 * agb::kTM;
     p.k_stride = ceil_div(hidden, 8) * 8;
     p.piece = ceil_div(vocab, 256) * 256;
     auto limit = [&](int64_t bytes_per_column, int64_t bytes) {
@@ -238,7 +239,8 @@ CePlan plan_ce(bool backward, int64_t rows, int64_t hidden, int64_t vocab, int d
     p.pieces = ceil_div(vocab, p.piece);
     p.g_stride = p.piece;
     p.dh_stride = ceil_div(hidden, 4) * 4;
-    p.pairs = p.pieces * (p.piece / 128);
+    p.tn = 256;
+    p.pairs = p.pieces * (p.piece / (p.tn / 2));
     // dh: few tiles with a long sum are cut along it, until the GPU has two per SM or a part has 16 slabs
     const int64_t tiles = p.rows_pad / agb::kTM * ceil_div(hidden, agb::kTN), blocks = ceil_div(p.piece, agb::kTK);
     int64_t s = ceil_div(2 * sms, tiles);
@@ -357,6 +359,9 @@ agb::CeArgs ce_args(const CeCall& c) {
     a.hidden = static_cast<int>(c.hidden);
     return a;
 }
+// Rows that fit one CTA's half of a pair's tile leave nothing for the other to do.
+int pair_size(const CeCall& c) { return c.rows <= agb::kTM ? 1 : 2; }
+
 // The logits of a piece: rows that take part x n columns.
 agb::CeJob logits_job(const CeCall& c, int epi, int64_t col0, int64_t n) {
     agb::CeJob j{};
@@ -368,19 +373,37 @@ agb::CeJob logits_job(const CeCall& c, int epi, int64_t col0, int64_t n) {
     j.k = static_cast<int>(c.hidden);
     j.splits = 1;
     j.k_per_split = static_cast<int>(ceil_div(c.hidden, agb::kTK) * agb::kTK);
+    j.tn = c.p.tn;
+    j.b_box = j.tn / pair_size(c) < 128 ? 64 : 128;
     return j;
 }
-int launch_gemm(const CeCall& c, const agb::CeArgs& a) {
+template <int CG>
+int launch_gemm_cg(const CeCall& c, const agb::CeArgs& a) {
     int64_t tiles = 0;
     for (int i = 0; i < a.jobs; ++i) {
         const agb::CeJob& j = a.job[i];
-        tiles += ceil_div(j.m < 0 ? c.rows : j.m, agb::kTM) * ceil_div(j.n, agb::kTN) * j.splits;
+        tiles += ceil_div(j.m < 0 ? c.rows : j.m, CG * agb::kTM) * ceil_div(j.n, j.tn) * j.splits;
     }
     if (tiles >= (1LL << 31)) return fail(AGB_ERR_UNSUPPORTED, "too many tiles");
-    AGB_CUDA(cudaFuncSetAttribute(agb::ce_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, agb::kCeSmem));
-    const unsigned grid = static_cast<unsigned>(tiles < c.d.sms ? tiles : c.d.sms);
-    agb::ce_gemm_kernel<<<grid, agb::kCeThreads, agb::kCeSmem, c.st>>>(a);
+    AGB_CUDA(cudaFuncSetAttribute(agb::ce_gemm_kernel<CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, agb::CeRing<CG>::kSmem));
+    const int64_t most = c.d.sms / CG;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>((tiles < most ? tiles : most) * CG));
+    cfg.blockDim = dim3(agb::kCeThreads);
+    cfg.dynamicSmemBytes = agb::CeRing<CG>::kSmem;
+    cfg.stream = c.st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CG;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    AGB_CUDA(cudaLaunchKernelEx(&cfg, agb::ce_gemm_kernel<CG>, a));
     return after_launch("linear_ce_gemm");
+}
+int launch_gemm(const CeCall& c, const agb::CeArgs& a) {
+    return pair_size(c) == 1 ? launch_gemm_cg<1>(c, a) : launch_gemm_cg<2>(c, a);
 }
 
 int start_ce(CeCall* c, bool backward, bool want_dh, void* workspace, size_t workspace_bytes, agb_stream_t stream) {
@@ -423,18 +446,18 @@ int agb_linear_ce_fwd(const void* h, const void* w, const void* target, int targ
         const int64_t col0 = i * c.p.piece, n = vocab - col0 < c.p.piece ? vocab - col0 : c.p.piece;
         AGB_TRY(ce_pack(c, col0, n));
         agb::CeArgs a = ce_args(c);
-        AGB_TRY(map_h(c, &a.A[0], 128));
-        AGB_TRY(map_w(c, &a.B[0], n, 128));
         a.jobs = 1;
         a.job[0] = logits_job(c, agb::kEpiPairs, col0, n);
+        AGB_TRY(map_h(c, &a.A[0], 128));
+        AGB_TRY(map_w(c, &a.B[0], n, a.job[0].b_box));
         a.pairs = c.at<float2>(c.p.pair_at);
         a.z_target = c.at<float>(c.p.z_target);
         a.col0 = static_cast<int>(col0);
-        a.pair0 = static_cast<int>(col0 / 128);
+        a.pair0 = static_cast<int>(col0 / (c.p.tn / 2));
         AGB_TRY(launch_gemm(c, a));
     }
     const int64_t last = vocab - (c.p.pieces - 1) * c.p.piece;
-    const int pairs = static_cast<int>((c.p.pieces - 1) * (c.p.piece / 128) + ceil_div(last, agb::kTN) * 2);
+    const int pairs = static_cast<int>((c.p.pieces - 1) * (c.p.piece / (c.p.tn / 2)) + ceil_div(last, c.p.tn) * 2);
     agb::ce_join_kernel<<<static_cast<unsigned>(ceil_div(rows, 32)), dim3(32, 8), 0, c.st>>>(
         c.at<float2>(c.p.pair_at), pairs, c.p.rows_pad, c.at<int>(c.p.count), c.at<float>(c.p.z_target), c.at<int>(c.p.row_of), loss, lse);
     return after_launch("linear_ce_join");
@@ -463,10 +486,10 @@ int agb_linear_ce_bwd(const void* h, const void* w, const void* target, int targ
         const int64_t col0 = i * c.p.piece, n = vocab - col0 < c.p.piece ? vocab - col0 : c.p.piece;
         AGB_TRY(ce_pack(c, col0, n));
         agb::CeArgs a = ce_args(c);
-        AGB_TRY(map_h(c, &a.A[0], 128));
-        AGB_TRY(map_w(c, &a.B[0], n, 128));
         a.jobs = 1;
         a.job[0] = logits_job(c, agb::kEpiG, col0, n);
+        AGB_TRY(map_h(c, &a.A[0], 128));
+        AGB_TRY(map_w(c, &a.B[0], n, a.job[0].b_box));
         a.col0 = static_cast<int>(col0);
         a.lse = c.at<float>(c.p.lse_of);
         a.gy = c.at<float>(c.p.gy_of);
@@ -487,6 +510,8 @@ int agb_linear_ce_bwd(const void* h, const void* w, const void* target, int targ
             j.splits = c.p.splits;
             j.k_per_split = c.p.k_per_split;
             j.n_first = 1;
+            j.tn = agb::kTN;
+            j.b_box = 64;
             AGB_TRY(map_g(c, &a.A[a.jobs], 128));
             AGB_TRY(map_w(c, &a.B[a.jobs], n, 64));
             a.dh = c.at<float>(c.p.dh);
@@ -506,6 +531,8 @@ int agb_linear_ce_bwd(const void* h, const void* w, const void* target, int targ
             j.splits = 1;
             j.k_per_split = static_cast<int>(c.p.rows_pad);
             j.n_first = 1;
+            j.tn = agb::kTN;
+            j.b_box = 64;
             AGB_TRY(map_g(c, &a.A[a.jobs], 64));
             AGB_TRY(map_h(c, &a.B[a.jobs], 64));
             a.dw = dw;

@@ -21,12 +21,17 @@
 
 namespace agb {
 
-constexpr int kTM = 128, kTN = 256, kTK = 64;
-constexpr int kStages = 4;
-constexpr int kBytesA = kTM * kTK * 2, kBytesB = kTN * kTK * 2;
-constexpr int kStageBytes = kBytesA + kBytesB;
-constexpr int kCeSmem = kStages * kStageBytes + 1024;
+constexpr int kTM = 128, kTN = 256, kTK = 64;          // rows of A per CTA, most columns of a tile, depth of a slab
 constexpr int kCeThreads = 384;        // TMA, MMA, TMEM, idle, and eight warps of epilogue
+// CG CTAs work on a tile of CG * 128 rows together (tcgen05 cta_group): each holds its 128 rows of A, its share of the columns of
+// B and the accumulators of its rows.  A pair reads half of B per CTA, so its ring is deeper for the same bytes.
+template <int CG>
+struct CeRing {
+    static constexpr int kStages = CG == 1 ? 4 : 6;
+    static constexpr int kBytesA = kTM * kTK * 2, kBytesB = kTN / CG * kTK * 2;
+    static constexpr int kStageBytes = kBytesA + kBytesB;
+    static constexpr int kSmem = kStages * kStageBytes + 1024;
+};
 
 // What an epilogue does with its tile.
 enum CeEpi { kEpiPairs = 0, kEpiG = 1, kEpiDh = 2, kEpiDw = 3 };
@@ -37,9 +42,11 @@ struct CeJob {
     int a_planes3, b_row0, a_row0;     // a_planes3: the six products of split fp32 operands; row offsets of the piece in B (A)
     int m, n, k;                       // extents; m < 0 or k < 0: the number of rows that take part, read on the device
     int splits, k_per_split;           // K cut into `splits` parts of k_per_split (a multiple of kTK)
-    int n_first;                       // tile order: 1 N fastest, 0 M fastest in groups of kMGroup tiles
+    int n_first;                       // tile order: 1 N fastest, 0 M fastest in groups of kMGroup rows
+    int tn;                            // columns of a tile: 256, 128 or 64 (a pair: 256)
+    int b_box;                         // rows of B's TMA box: 64 where B is MN-major, else 128 or a CTA's whole share
 };
-constexpr int kMGroup = 32;
+constexpr int kMGroup = 4096;
 
 struct CeArgs {
     CUtensorMap A[2], B[2];
@@ -74,13 +81,14 @@ struct CeTile {
 
 // The extents of a job with the device's row count filled in, and its number of tiles.
 struct CeShape {
-    int m, n, k, mt, nt, tiles;
-    __device__ __forceinline__ CeShape(const CeJob& j, int count) {
+    int m, n, k, tm, mt, nt, tiles;
+    __device__ __forceinline__ CeShape(const CeJob& j, int count, int tile_m) {
         m = j.m < 0 ? count : j.m;
         k = j.k < 0 ? count : j.k;
         n = j.n;
-        mt = (m + kTM - 1) / kTM;
-        nt = (n + kTN - 1) / kTN;
+        tm = tile_m;
+        mt = (m + tm - 1) / tm;
+        nt = (n + j.tn - 1) / j.tn;
         tiles = mt * nt * j.splits;
     }
 };
@@ -93,14 +101,14 @@ __device__ __forceinline__ CeTile ce_tile(const CeJob& j, const CeShape& s, int 
         n = t % s.nt;
         m = t / s.nt;
     } else {
-        const int group = t / (kMGroup * s.nt), first = group * kMGroup;
-        const int height = s.mt - first < kMGroup ? s.mt - first : kMGroup;
-        t -= group * kMGroup * s.nt;
+        const int tall = kMGroup / s.tm, group = t / (tall * s.nt), first = group * tall;
+        const int height = s.mt - first < tall ? s.mt - first : tall;
+        t -= first * s.nt;
         m = first + t % height;
         n = t / height;
     }
-    o.m0 = m * kTM;
-    o.n0 = n * kTN;
+    o.m0 = m * s.tm;
+    o.n0 = n * j.tn;
     o.k0 = o.split * j.k_per_split;
     const int k1 = o.k0 + j.k_per_split < s.k ? o.k0 + j.k_per_split : s.k;
     const int blocks = k1 > o.k0 ? (k1 - o.k0 + kTK - 1) / kTK : 0;
@@ -242,13 +250,17 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const T* w, int64_t rows, 
 }
 
 // ---------------------------------------------------------------- the products
+template <int CG>
 __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_constant__ CeArgs a) {
+    typedef CeRing<CG> R;
+    constexpr int kStages = R::kStages;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], drained;
     __shared__ uint32_t tmem_base;
     __shared__ volatile int abort_flag;
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = CG == 1 ? 0 : static_cast<int>(cluster_rank());
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&full[s], 1);
@@ -256,120 +268,143 @@ __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_con
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&acc_full[i], 1);
-            mbar_init(&acc_empty[i], 8);
+            mbar_init(&acc_empty[i], 8 * CG);
         }
         mbar_init(&drained, 1);
         abort_flag = 0;
         mbar_fence_init();
     }
-    if (warp == 2) tmem_alloc(&tmem_base, 512);
+    if (warp == 2) tmem_alloc<CG>(&tmem_base, 512);
     tc_fence_before();
     __syncthreads();
+    if (CG == 2) cluster_barrier();                    // the leader's barriers are ready before the other CTA's copies arrive
     tc_fence_after();
     const uint32_t tmem = tmem_base;
     const int count = *a.count;
-    const CeShape s0(a.job[0], count), s1(a.job[a.jobs - 1], count);
+    const CeShape s0(a.job[0], count, kTM * CG), s1(a.job[a.jobs - 1], count, kTM * CG);
     const int total = s0.tiles + (a.jobs > 1 ? s1.tiles : 0);
+    const int first = blockIdx.x / CG, stride = gridDim.x / CG;
 
     if (warp == 0) {
         if (lane == 0) {
-            int fills = 0;
+            const uint32_t full0 = leader_address(&full[0]);
+            int fills = 0, s = 0;                      // s: slot of the ring
+            uint32_t wrap = 1;                         // parity of the slot's previous use
             bool ok = true;
-            for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+            for (int t = first; t < total && ok; t += stride) {
                 const int j = t < s0.tiles ? 0 : 1;
-                const CeJob& job = a.job[j];
-                const CeTile tile = ce_tile(job, j ? s1 : s0, j ? t - s0.tiles : t);
-                const int blocks = job.a_planes3 ? tile.iters / 6 : tile.iters;
-                for (int it = 0; it < tile.iters && ok; ++it, ++fills) {
-                    const int s = fills % kStages;
-                    if (fills >= kStages && !wait_or_abort(&empty[s], (fills / kStages - 1) & 1, &abort_flag, a.status)) {
-                        ok = false;
-                        break;
-                    }
+                const CeTile tile = ce_tile(a.job[j], j ? s1 : s0, j ? t - s0.tiles : t);
+                // everything that the inner loop needs, in registers: one thread feeds the tensor cores of the CTA, and a
+                // division or a load from the argument's memory per slab cost it more than the slab's products take
+                const bool a_mn = a.job[j].a_mn, b_mn = a.job[j].b_mn;
+                const int share = a.job[j].tn / CG;                     // columns of B that this CTA holds
+                const int box = a.job[j].b_box, boxes = share / box;
+                const int am = (a_mn ? a.job[j].a_row0 : 0) + tile.m0 + rank * kTM;
+                const int b_row0 = a.job[j].b_row0, bn = tile.n0 + rank * share;
+                const uint32_t bytes = CG * (R::kBytesA + share * kTK * 2);
+                const CUtensorMap* ma = &a.A[j];
+                const CUtensorMap* mb = &a.B[j];
+                const int products = a.job[j].a_planes3 ? 6 : 1, blocks = tile.iters / products;
+                for (int p = 0; p < products && ok; ++p) {
                     int pa = 0, pb = 0;
-                    if (job.a_planes3) plane_pair(it / blocks, pa, pb);
-                    const int k = tile.k0 + (it % blocks) * kTK;
-                    uint8_t* sa = ring + s * kStageBytes;
-                    uint8_t* sb = sa + kBytesA;
-                    mbar_arrive_expect_tx(&full[s], kStageBytes);
-                    if (job.a_mn) {
+                    if (products == 6) plane_pair(p, pa, pb);
+                    int k = tile.k0;
+                    for (int it = 0; it < blocks; ++it, ++fills, k += kTK) {
+                        if (fills >= kStages && !wait_or_abort(&empty[s], wrap, &abort_flag, a.status)) {
+                            ok = false;
+                            break;
+                        }
+                        uint8_t* sa = ring + s * R::kStageBytes;
+                        uint8_t* sb = sa + R::kBytesA;
+                        const uint32_t bar = CG == 1 ? smem_u32(&full[s]) : full0 + s * 8;
+                        if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);     // both CTAs' bytes
+                        if (a_mn) {
 #pragma unroll
-                        for (int b = 0; b < kTM / 64; ++b)
-                            tma_load_3d(sa + b * (kTK * 128), &a.A[j], job.a_row0 + tile.m0 + b * 64, k, pa, &full[s]);
-                    } else {
-                        tma_load_3d(sa, &a.A[j], k, tile.m0, pa, &full[s]);
-                    }
-                    if (job.b_mn) {
-#pragma unroll
-                        for (int b = 0; b < kTN / 64; ++b)
-                            tma_load_3d(sb + b * (kTK * 128), &a.B[j], tile.n0 + b * 64, job.b_row0 + k, pb, &full[s]);
-                    } else {
-#pragma unroll
-                        for (int b = 0; b < kTN / 128; ++b)
-                            tma_load_3d(sb + b * (128 * 128), &a.B[j], k, job.b_row0 + tile.n0 + b * 128, pb, &full[s]);
+                            for (int b = 0; b < kTM / 64; ++b) tma_load_3d<CG>(sa + b * (kTK * 128), ma, am + b * 64, k, pa, bar);
+                        } else {
+                            tma_load_3d<CG>(sa, ma, k, am, pa, bar);
+                        }
+                        if (b_mn) {
+                            for (int b = 0; b < boxes; ++b) tma_load_3d<CG>(sb + b * (kTK * 128), mb, bn + b * 64, b_row0 + k, pb, bar);
+                        } else {
+                            for (int b = 0; b < boxes; ++b) tma_load_3d<CG>(sb + b * box * 128, mb, k, b_row0 + bn + b * box, pb, bar);
+                        }
+                        if (++s == kStages) {
+                            s = 0;
+                            wrap ^= 1;
+                        }
                     }
                 }
             }
-            if (!ok)                                   // the copies still in flight land before the CTA leaves
-                for (int f = fills > kStages ? fills - kStages : 0; f < fills; ++f) mbar_wait_bounded(&full[f % kStages], (f / kStages) & 1);
+            if (!ok) {                                 // the copies still in flight land before the CTA leaves
+                if (CG == 1)
+                    for (int f = fills > kStages ? fills - kStages : 0; f < fills; ++f) mbar_wait_bounded(&full[f % kStages], (f / kStages) & 1);
+                else
+                    for (int i = 0; i < 2000; ++i) __nanosleep(1000);   // counted on the leader's barrier: given two milliseconds
+            }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            int uses = 0, n = 0;
+        if (lane == 0 && rank == 0) {
+            int n = 0, s = 0;
+            uint32_t phase = 0;
             bool ok = true;
-            for (int t = blockIdx.x; t < total && ok; t += gridDim.x, ++n) {
+            const uint32_t ring0 = smem_u32(ring);
+            const uint64_t desc = smem_desc(0, kTK * 128);
+            for (int t = first; t < total && ok; t += stride, ++n) {
                 const int j = t < s0.tiles ? 0 : 1;
-                const CeJob& job = a.job[j];
-                const CeTile tile = ce_tile(job, j ? s1 : s0, j ? t - s0.tiles : t);
-                const uint32_t idesc = mma_idesc(kTM, kTN, job.a_mn, job.b_mn);
-                const int acc = n & 1;
+                const CeTile tile = ce_tile(a.job[j], j ? s1 : s0, j ? t - s0.tiles : t);
+                const uint32_t idesc = mma_idesc(kTM * CG, a.job[j].tn, a.job[j].a_mn, a.job[j].b_mn);
+                const uint32_t step_a = (a.job[j].a_mn ? 2048 : 32) >> 4, step_b = (a.job[j].b_mn ? 2048 : 32) >> 4;
+                const int acc = n & 1, iters = tile.iters;
                 if (n >= 2 && !wait_or_abort(&acc_empty[acc], (n / 2 - 1) & 1, &abort_flag, a.status)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
                 const uint32_t d = tmem + acc * kTN;
-                const uint32_t step_a = job.a_mn ? 2048 : 32, step_b = job.b_mn ? 2048 : 32;
-                for (int it = 0; it < tile.iters; ++it, ++uses) {
-                    const int s = uses % kStages;
-                    if (!wait_or_abort(&full[s], (uses / kStages) & 1, &abort_flag, a.status)) {
+                for (int it = 0; it < iters; ++it) {
+                    if (!wait_or_abort(&full[s], phase, &abort_flag, a.status)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t sa = smem_u32(ring + s * kStageBytes), sb = sa + kBytesA;
+                    const uint64_t da = desc + ((ring0 + s * R::kStageBytes) >> 4), db = da + (R::kBytesA >> 4);
 #pragma unroll
-                    for (int k = 0; k < kTK / 16; ++k)
-                        mma_bf16(d, smem_desc(sa + k * step_a, kTK * 128), smem_desc(sb + k * step_b, kTK * 128), idesc, it > 0 || k > 0);
-                    mma_commit(&empty[s]);
+                    for (int k = 0; k < kTK / 16; ++k) mma_bf16<CG>(d, da + k * step_a, db + k * step_b, idesc, it > 0 || k > 0);
+                    mma_commit<CG>(&empty[s]);
+                    if (++s == kStages) {
+                        s = 0;
+                        phase ^= 1;
+                    }
                 }
-                mma_commit(&acc_full[acc]);
+                mma_commit<CG>(&acc_full[acc]);
             }
             if (!ok) {
-                mma_commit(&drained);
+                mma_commit<CG>(&drained);
                 mbar_wait_bounded(&drained, 0);
             }
         }
     } else if (warp >= 4) {
-        const int quarter = warp & 3, part = (warp - 4) >> 2;     // lanes 32 * quarter.., columns 128 * part..
+        const int quarter = warp & 3, part = (warp - 4) >> 2;     // lanes 32 * quarter.., the part-th half of the columns
+        const uint32_t acc_empty_at[2] = {leader_address(&acc_empty[0]), leader_address(&acc_empty[1])};
         int n = 0;
-        for (int t = blockIdx.x; t < total; t += gridDim.x, ++n) {
+        for (int t = first; t < total; t += stride, ++n) {
             const int j = t < s0.tiles ? 0 : 1;
             const CeJob& job = a.job[j];
             const CeShape& sh = j ? s1 : s0;
             const CeTile tile = ce_tile(job, sh, j ? t - s0.tiles : t);
-            const int acc = n & 1;
+            const int acc = n & 1, width = job.tn >> 1;
             if (!wait_or_abort(&acc_full[acc], (n / 2) & 1, &abort_flag, a.status)) break;
             tc_fence_after();
-            const uint32_t d = tmem + acc * kTN + part * 128 + (static_cast<uint32_t>(quarter * 32) << 16);
-            const int row = tile.m0 + quarter * 32 + lane;
+            const uint32_t d = tmem + acc * kTN + part * width + (static_cast<uint32_t>(quarter * 32) << 16);
+            const int row = tile.m0 + rank * kTM + quarter * 32 + lane;
             const bool live = row < sh.m;
             const bool empty_sum = tile.iters == 0;    // nothing was multiplied: the accumulators hold something old
-            const int c0 = tile.n0 + part * 128;
+            const int c0 = tile.n0 + part * width;
             if (job.epi == kEpiPairs) {
                 float m = -INFINITY, s = 0.f;
                 const int tgt = live ? a.target[row] - a.col0 : -1;
-                for (int c = c0; c < c0 + 128; c += 32) {
+                for (int c = c0; c < c0 + width; c += 32) {
                     float v[32];
                     tmem_load32(d + (c - c0), v);
                     const int left = sh.n - c;
@@ -387,13 +422,13 @@ __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_con
                     }
                     online_add(v, 1.f, m, s);
                 }
-                if (live) a.pairs[static_cast<int64_t>(a.pair0 + c0 / 128) * a.rows_pad + row] = make_float2(m, s);
+                if (live) a.pairs[static_cast<int64_t>(a.pair0 + c0 / width) * a.rows_pad + row] = make_float2(m, s);
             } else if (job.epi == kEpiG) {
                 const int tgt = live ? a.target[row] - a.col0 : -1;
                 const float lse = live ? a.lse[row] : 0.f, gy = live ? a.gy[row] : 0.f;
                 __nv_bfloat16* out = a.g + row * a.g_stride;
                 const int64_t plane = a.rows_pad * a.g_stride;
-                for (int c = c0; c < c0 + 128; c += 32) {
+                for (int c = c0; c < c0 + width; c += 32) {
                     float v[32];
                     tmem_load32(d + (c - c0), v);
 #pragma unroll
@@ -419,7 +454,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_con
                 }
             } else if (job.epi == kEpiDh) {
                 float* out = a.dh + (static_cast<int64_t>(tile.split) * a.rows_pad + row) * a.dh_stride;
-                for (int c = c0; c < c0 + 128 && c < sh.n; c += 32) {
+                for (int c = c0; c < c0 + width && c < sh.n; c += 32) {
                     float v[32];
                     tmem_load32(d + (c - c0), v);
                     if (!live) continue;
@@ -438,7 +473,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_con
             } else {
                 const int64_t at = static_cast<int64_t>(a.col0 + row) * a.hidden;
                 const bool vec = a.hidden % 8 == 0 && (reinterpret_cast<uintptr_t>(a.dw) & 15) == 0;
-                for (int c = c0; c < c0 + 128 && c < sh.n; c += 32) {
+                for (int c = c0; c < c0 + width && c < sh.n; c += 32) {
                     float v[32];
                     tmem_load32(d + (c - c0), v);
                     if (!live) continue;
@@ -477,14 +512,18 @@ __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_con
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[acc]);
+            if (lane == 0) {
+                if (CG == 1) mbar_arrive(&acc_empty[acc]);
+                else mbar_arrive_cluster(acc_empty_at[acc]);
+            }
         }
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if (CG == 2) cluster_barrier();                    // neither CTA leaves while the other may still reach its memory
     tc_fence_after();
-    if (warp == 2) tmem_free(tmem, 512);
+    if (warp == 2) tmem_free<CG>(tmem, 512);
 }
 
 // ---------------------------------------------------------------- joining
