@@ -215,10 +215,33 @@ struct CePlan {
     int planes;
     bool direct_w;              // TMA reads W as it is
     int64_t rows_pad, k_stride, piece, pieces, g_stride, dh_stride, pairs;
+    int pair;                   // CTAs that work on a tile together
     int tn;                     // columns of a tile of logits
+    int64_t pairs_per_piece;
     int splits, k_per_split;
-    size_t h, w, count, row_of, pos_of, target_of, lse_of, gy_of, z_target, pair_at, g, dh, total;
+    size_t h, w, count, row_of, pos_of, target_of, lse_of, gy_of, left_over, z_target, pair_at, g, dh, total;
 };
+
+// Columns of a tile of logits.  A slab of a tile takes the longest of its products (2 clocks per column), its bytes from L2 at 64 a
+// clock, and its share of W from memory at 24 a clock (the measured rate over the SMs), which the tiles above it share; what counts is
+// that times the turns that the GPU takes.  16 x 4096 x 32768: one turn of 147 tiles of 224 columns instead of one of 128 tiles of 256.
+int choose_tn(int pair, int64_t rows, int64_t columns, int step, int sms) {
+    const int64_t mt = ceil_div(rows, pair * agb::kTM), units = sms / pair;
+    int best = 256;
+    double least = 0;
+    for (int tn = 256; tn >= 64; tn -= step) {
+        double slab = 2.0 * tn;
+        const double l2 = (agb::kTM * 128 + tn / pair * 128) / 64.0, dram = tn / pair * 128 / 24.0 / static_cast<double>(mt);
+        if (l2 > slab) slab = l2;
+        if (dram > slab) slab = dram;
+        const double cost = slab * static_cast<double>(ceil_div(mt * ceil_div(columns, tn), units));
+        if (tn == 256 || cost < 0.97 * least) {
+            best = tn;
+            least = cost;
+        }
+    }
+    return best;
+}
 
 CePlan plan_ce(bool backward, int64_t rows, int64_t hidden, int64_t vocab, int dtype, bool want_dh, int sms) {
     CePlan p{};
@@ -239,8 +262,10 @@ CePlan plan_ce(bool backward, int64_t rows, int64_t hidden, int64_t vocab, int d
     p.pieces = ceil_div(vocab, p.piece);
     p.g_stride = p.piece;
     p.dh_stride = ceil_div(hidden, 4) * 4;
-    p.tn = 256;
-    p.pairs = p.pieces * (p.piece / (p.tn / 2));
+    p.pair = rows <= agb::kTM ? 1 : 2;     // rows that fit one CTA's half of a pair's tile leave nothing for the other to do
+    p.tn = choose_tn(p.pair, rows, p.piece < vocab ? p.piece : vocab, backward ? 64 : 32, sms);
+    p.pairs_per_piece = ceil_div(p.piece, p.tn) * 2;
+    p.pairs = p.pieces * p.pairs_per_piece;
     // dh: few tiles with a long sum are cut along it, until the GPU has two per SM or a part has 16 slabs
     const int64_t tiles = p.rows_pad / agb::kTM * ceil_div(hidden, agb::kTN), blocks = ceil_div(p.piece, agb::kTK);
     int64_t s = ceil_div(2 * sms, tiles);
@@ -262,6 +287,7 @@ CePlan plan_ce(bool backward, int64_t rows, int64_t hidden, int64_t vocab, int d
     if (backward) {
         take(&p.lse_of, p.rows_pad * 4);
         take(&p.gy_of, p.rows_pad * 4);
+        take(&p.left_over, p.rows_pad * 4);
         take(&p.g, static_cast<size_t>(p.planes) * p.rows_pad * p.g_stride * 2);
         if (want_dh) take(&p.dh, static_cast<size_t>(p.splits) * p.rows_pad * p.dh_stride * 4);
     } else {
@@ -320,7 +346,9 @@ int ce_rows(const CeCall& c, const float* lse, const float* gy, float* loss, flo
     }
     a.loss = loss;
     a.lse_out = lse_out;
-    const unsigned grid = static_cast<unsigned>(ceil_div(c.rows, agb::kRowsBlock));
+    // a warp per row while the blocks, which all count the targets before their own, stay about a thousand
+    a.per_block = c.rows <= 8192 ? 8 : c.rows <= 16384 ? 16 : agb::kRowsBlock;
+    const unsigned grid = static_cast<unsigned>(ceil_div(c.rows, a.per_block));
     if (c.dtype == AGB_F32) agb::ce_rows_kernel<float><<<grid, 256, 0, c.st>>>(a);
     else agb::ce_rows_kernel<bf16><<<grid, 256, 0, c.st>>>(a);
     return after_launch("linear_ce_rows");
@@ -359,9 +387,6 @@ agb::CeArgs ce_args(const CeCall& c) {
     a.hidden = static_cast<int>(c.hidden);
     return a;
 }
-// Rows that fit one CTA's half of a pair's tile leave nothing for the other to do.
-int pair_size(const CeCall& c) { return c.rows <= agb::kTM ? 1 : 2; }
-
 // The logits of a piece: rows that take part x n columns.
 agb::CeJob logits_job(const CeCall& c, int epi, int64_t col0, int64_t n) {
     agb::CeJob j{};
@@ -374,7 +399,7 @@ agb::CeJob logits_job(const CeCall& c, int epi, int64_t col0, int64_t n) {
     j.splits = 1;
     j.k_per_split = static_cast<int>(ceil_div(c.hidden, agb::kTK) * agb::kTK);
     j.tn = c.p.tn;
-    j.b_box = j.tn / pair_size(c) < 128 ? 64 : 128;
+    j.b_box = j.tn / c.p.pair;
     return j;
 }
 template <int CG>
@@ -403,7 +428,7 @@ int launch_gemm_cg(const CeCall& c, const agb::CeArgs& a) {
     return after_launch("linear_ce_gemm");
 }
 int launch_gemm(const CeCall& c, const agb::CeArgs& a) {
-    return pair_size(c) == 1 ? launch_gemm_cg<1>(c, a) : launch_gemm_cg<2>(c, a);
+    return c.p.pair == 1 ? launch_gemm_cg<1>(c, a) : launch_gemm_cg<2>(c, a);
 }
 
 int start_ce(CeCall* c, bool backward, bool want_dh, void* workspace, size_t workspace_bytes, agb_stream_t stream) {
@@ -453,13 +478,21 @@ int agb_linear_ce_fwd(const void* h, const void* w, const void* target, int targ
         a.pairs = c.at<float2>(c.p.pair_at);
         a.z_target = c.at<float>(c.p.z_target);
         a.col0 = static_cast<int>(col0);
-        a.pair0 = static_cast<int>(col0 / (c.p.tn / 2));
+        a.n_pairs = c.p.pairs;
+        a.pair0 = static_cast<int>(i * c.p.pairs_per_piece);
         AGB_TRY(launch_gemm(c, a));
     }
     const int64_t last = vocab - (c.p.pieces - 1) * c.p.piece;
-    const int pairs = static_cast<int>((c.p.pieces - 1) * (c.p.piece / (c.p.tn / 2)) + ceil_div(last, c.p.tn) * 2);
-    agb::ce_join_kernel<<<static_cast<unsigned>(ceil_div(rows, 32)), dim3(32, 8), 0, c.st>>>(
-        c.at<float2>(c.p.pair_at), pairs, c.p.rows_pad, c.at<int>(c.p.count), c.at<float>(c.p.z_target), c.at<int>(c.p.row_of), loss, lse);
+    const int pairs = static_cast<int>((c.p.pieces - 1) * c.p.pairs_per_piece + ceil_div(last, c.p.tn) * 2);
+    const unsigned grid = static_cast<unsigned>(ceil_div(rows, 8));
+    if (dtype == AGB_F32)
+        agb::ce_join_kernel<float><<<grid, 256, 0, c.st>>>(c.at<float2>(c.p.pair_at), pairs, c.p.pairs, c.at<int>(c.p.count), c.at<float>(c.p.z_target),
+                                                           c.at<int>(c.p.target_of), c.at<int>(c.p.row_of), static_cast<const float*>(h),
+                                                           static_cast<const float*>(w), (int)hidden, loss, lse);
+    else
+        agb::ce_join_kernel<bf16><<<grid, 256, 0, c.st>>>(c.at<float2>(c.p.pair_at), pairs, c.p.pairs, c.at<int>(c.p.count), c.at<float>(c.p.z_target),
+                                                          c.at<int>(c.p.target_of), c.at<int>(c.p.row_of), static_cast<const bf16*>(h),
+                                                          static_cast<const bf16*>(w), (int)hidden, loss, lse);
     return after_launch("linear_ce_join");
 }
 
@@ -495,6 +528,9 @@ int agb_linear_ce_bwd(const void* h, const void* w, const void* target, int targ
         a.gy = c.at<float>(c.p.gy_of);
         a.g = c.at<bf16>(c.p.g);
         a.g_stride = c.p.g_stride;
+        a.left_over = c.p.planes == 1 ? c.at<float>(c.p.left_over) : nullptr;
+        a.h = c.at<bf16>(c.p.h);
+        a.h_stride = c.p.k_stride;
         AGB_TRY(launch_gemm(c, a));
         a.jobs = 0;
         if (dh) {
@@ -543,13 +579,16 @@ int agb_linear_ce_bwd(const void* h, const void* w, const void* target, int targ
         AGB_TRY(launch_gemm(c, a));
     }
     if (dh) {
-        const unsigned grid = static_cast<unsigned>(rows < 16LL * c.d.sms ? rows : 16LL * c.d.sms);
+        const dim3 grid(static_cast<unsigned>(ceil_div(ceil_div(hidden, 4), 256)), static_cast<unsigned>(rows < 32768 ? rows : 32768));
+        const float* left = c.p.planes == 1 ? c.at<float>(c.p.left_over) : nullptr;
         if (dtype == AGB_F32)
             agb::ce_dh_kernel<float><<<grid, 256, 0, c.st>>>(c.at<float>(c.p.dh), c.p.splits, c.p.rows_pad, c.p.dh_stride, c.at<int>(c.p.pos_of),
-                                                             static_cast<float*>(dh), rows, (int)hidden);
+                                                             c.at<int>(c.p.target_of), left, static_cast<const float*>(w), static_cast<float*>(dh),
+                                                             rows, (int)hidden);
         else
             agb::ce_dh_kernel<bf16><<<grid, 256, 0, c.st>>>(c.at<float>(c.p.dh), c.p.splits, c.p.rows_pad, c.p.dh_stride, c.at<int>(c.p.pos_of),
-                                                            static_cast<bf16*>(dh), rows, (int)hidden);
+                                                            c.at<int>(c.p.target_of), left, static_cast<const bf16*>(w), static_cast<bf16*>(dh),
+                                                            rows, (int)hidden);
         return after_launch("linear_ce_dh");
     }
     return AGB_OK;

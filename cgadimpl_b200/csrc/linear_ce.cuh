@@ -25,12 +25,16 @@ constexpr int kTM = 128, kTN = 256, kTK = 64;          // rows of A per CTA, mos
 constexpr int kCeThreads = 384;        // TMA, MMA, TMEM, idle, and eight warps of epilogue
 // CG CTAs work on a tile of CG * 128 rows together (tcgen05 cta_group): each holds its 128 rows of A, its share of the columns of
 // B and the accumulators of its rows.  A pair reads half of B per CTA, so its ring is deeper for the same bytes.
+// Behind the ring each epilogue warp has 32 x 32 floats (rows 33 apart) through which a thread's run of columns becomes a row's: stores
+// of 64 bytes and more per row instead of 32 rows touched by each instruction.
+constexpr int kStageFloats = 32 * 33;
+constexpr int kHits = 16;
 template <int CG>
 struct CeRing {
     static constexpr int kStages = CG == 1 ? 4 : 6;
     static constexpr int kBytesA = kTM * kTK * 2, kBytesB = kTN / CG * kTK * 2;
     static constexpr int kStageBytes = kBytesA + kBytesB;
-    static constexpr int kSmem = kStages * kStageBytes + 1024;
+    static constexpr int kSmem = kStages * kStageBytes + 8 * kStageFloats * 4 + 1024;
 };
 
 // What an epilogue does with its tile.
@@ -43,8 +47,8 @@ struct CeJob {
     int m, n, k;                       // extents; m < 0 or k < 0: the number of rows that take part, read on the device
     int splits, k_per_split;           // K cut into `splits` parts of k_per_split (a multiple of kTK)
     int n_first;                       // tile order: 1 N fastest, 0 M fastest in groups of kMGroup rows
-    int tn;                            // columns of a tile: 256, 128 or 64 (a pair: 256)
-    int b_box;                         // rows of B's TMA box: 64 where B is MN-major, else 128 or a CTA's whole share
+    int tn;                            // columns of a tile, at most 256
+    int b_box;                         // rows of B's TMA box: 64 where B is MN-major, else a CTA's whole share of the columns
 };
 constexpr int kMGroup = 4096;
 
@@ -56,7 +60,8 @@ struct CeArgs {
     int* status;
     int64_t rows_pad;                  // row stride of the per-row arrays below
     // pairs
-    float2* pairs;                     // [half tiles of the vocabulary][rows_pad]
+    float2* pairs;                     // [rows_pad][half tiles of the vocabulary]
+    int64_t n_pairs;
     float* z_target;                   // [rows_pad]
     const int* target;                 // [rows_pad]
     int pair0;                         // first half tile of this piece
@@ -64,6 +69,7 @@ struct CeArgs {
     // g
     const float *lse, *gy;             // [rows_pad]
     __nv_bfloat16* g;                  // [planes][rows_pad][g_stride]
+    float* left_over;                  // [rows_pad]: what rounding took from g at the row's target (one plane only, else NULL)
     int64_t g_stride;
     int planes;
     // dh: fp32 parts [split][rows_pad][dh_stride]
@@ -72,6 +78,8 @@ struct CeArgs {
     int dh_add;                        // 0 the first piece: write, 1 add
     // dw
     void* dw;
+    const __nv_bfloat16* h;            // [rows_pad][h_stride], for what is left over
+    int64_t h_stride;
     int hidden, dw_add, dw_f32;
 };
 
@@ -140,13 +148,13 @@ __device__ __forceinline__ void split3(float x, uint32_t& hi, uint32_t& mid, uin
 // Rows of x [rows][cols] whose target names a column, in order and without gaps, into dst [planes][rows_pad][stride] bf16;
 // zeros behind the last column up to `stride` and, for the backward, behind the last row up to a multiple of kTK.  Also the
 // per-row arrays.
-// A block takes 32 rows; it counts the targets before its own to know where they go.
+// A block takes `per_block` (at most 32) rows; it counts the targets before its own to know where they go.
 struct CeRowsArgs {
     const void* x;
     const void* target;
     int target64;
     int64_t rows;
-    int cols, vocab, planes;
+    int cols, vocab, planes, per_block;
     __nv_bfloat16* dst;
     int64_t rows_pad, stride;
     int* count;
@@ -157,35 +165,57 @@ struct CeRowsArgs {
     float *lse_of, *gy_of;
     float *loss, *lse_out;             // forward: rows that take no part get 0
 };
-constexpr int kRowsBlock = 32;
+constexpr int kRowsBlock = 32;         // most rows of a block
 
 __device__ __forceinline__ int ce_target(const CeRowsArgs& a, int64_t r) {
     const int64_t t = a.target64 ? static_cast<const int64_t*>(a.target)[r] : static_cast<const int32_t*>(a.target)[r];
     return t >= 0 && t < a.vocab ? static_cast<int>(t) : -1;
 }
 
-// One row into its planes; `vec`: 16-byte loads are possible.
+// One row into its planes; `vec`: 16-byte loads are possible.  Loads are issued in batches before the stores that may alias them.
 template <typename T>
-__device__ __forceinline__ void ce_copy_row(const T* src, __nv_bfloat16* dst, int cols, int64_t stride, int64_t plane, bool vec, int lane,
-                                            int lanes) {
-    if (sizeof(T) == 2) {
-        if (vec) {
-            const uint4* s = reinterpret_cast<const uint4*>(src);
-            uint4* d = reinterpret_cast<uint4*>(dst);
-            for (int i = lane; i < cols / 8; i += lanes) d[i] = s[i];
-        } else {
-            const uint16_t* s = reinterpret_cast<const uint16_t*>(src);
-            uint16_t* d = reinterpret_cast<uint16_t*>(dst);
-            for (int i = lane; i < stride; i += lanes) d[i] = i < cols ? s[i] : static_cast<uint16_t>(0);
+__device__ __forceinline__ void ce_copy_row(const T* src, __nv_bfloat16* dst, int cols, int64_t stride, int64_t plane, bool vec, int lane) {
+    constexpr int B = 8;
+    if (sizeof(T) == 2 && vec) {
+        const uint4* s = reinterpret_cast<const uint4*>(src);
+        uint4* d = reinterpret_cast<uint4*>(dst);
+        const int n = cols / 8;
+        for (int i0 = lane; i0 < n; i0 += 32 * B) {
+            uint4 v[B];
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+                if (i0 + 32 * b < n) v[b] = s[i0 + 32 * b];
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+                if (i0 + 32 * b < n) d[i0 + 32 * b] = v[b];
         }
-    } else {
-        uint16_t* d = reinterpret_cast<uint16_t*>(dst);
-        for (int i = lane; i < stride; i += lanes) {
-            uint32_t hi = 0, mid = 0, lo = 0;
-            if (i < cols) split3(Vec<T>::load1(src + i), hi, mid, lo);
-            d[i] = static_cast<uint16_t>(hi >> 16);
-            d[plane + i] = static_cast<uint16_t>(mid >> 16);
-            d[2 * plane + i] = static_cast<uint16_t>(lo >> 16);
+        return;
+    }
+    uint32_t* d = reinterpret_cast<uint32_t*>(dst);    // two columns at a time: the stride is a multiple of 8
+    const int n = static_cast<int>(stride / 2);
+    const int64_t p32 = plane / 2;
+    for (int i0 = lane; i0 < n; i0 += 32 * B) {
+        T v[B][2];
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const int c = 2 * (i0 + 32 * b);
+            v[b][0] = c < cols ? src[c] : T(0.f);
+            v[b][1] = c + 1 < cols ? src[c + 1] : T(0.f);
+        }
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const int i = i0 + 32 * b;
+            if (i >= n) continue;
+            if (sizeof(T) == 2) {
+                d[i] = (__float_as_uint(Vec<T>::load1(&v[b][0])) >> 16) | (__float_as_uint(Vec<T>::load1(&v[b][1])) & 0xffff0000u);
+            } else {
+                uint32_t h0, m0, l0, h1, m1, l1;
+                split3(Vec<T>::load1(&v[b][0]), h0, m0, l0);
+                split3(Vec<T>::load1(&v[b][1]), h1, m1, l1);
+                d[i] = (h0 >> 16) | h1;
+                d[p32 + i] = (m0 >> 16) | m1;
+                d[2 * p32 + i] = (l0 >> 16) | l1;
+            }
         }
     }
 }
@@ -195,8 +225,9 @@ __global__ void __launch_bounds__(256) ce_rows_kernel(const CeRowsArgs a) {
     __shared__ int warp_count[8];
     __shared__ int where[kRowsBlock];
     __shared__ int last;
-    const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kRowsBlock;
+    const int64_t r0 = static_cast<int64_t>(blockIdx.x) * a.per_block;
     int n = 0;
+#pragma unroll 4
     for (int64_t r = threadIdx.x; r < r0; r += 256) n += ce_target(a, r) >= 0;
     n = __reduce_add_sync(0xffffffffu, n);
     if ((threadIdx.x & 31) == 0) warp_count[threadIdx.x >> 5] = n;
@@ -205,7 +236,7 @@ __global__ void __launch_bounds__(256) ce_rows_kernel(const CeRowsArgs a) {
     for (int w = 0; w < 8; ++w) base += warp_count[w];
     if (threadIdx.x < 32) {
         const int64_t r = r0 + threadIdx.x;
-        const int t = r < a.rows ? ce_target(a, r) : -1;
+        const int t = threadIdx.x < a.per_block && r < a.rows ? ce_target(a, r) : -1;
         const uint32_t mask = __ballot_sync(0xffffffffu, t >= 0);
         const int at = base + __popc(mask & ((1u << threadIdx.x) - 1));
         where[threadIdx.x] = t >= 0 ? at : -1;
@@ -216,20 +247,20 @@ __global__ void __launch_bounds__(256) ce_rows_kernel(const CeRowsArgs a) {
                 a.lse_of[at] = a.lse[r];
                 a.gy_of[at] = a.gy[r];
             }
-        } else if (r < a.rows && a.loss) {
+        } else if (threadIdx.x < a.per_block && r < a.rows && a.loss) {
             a.loss[r] = 0.f;
             a.lse_out[r] = 0.f;
         }
-        if (r < a.rows) a.pos_of[r] = t >= 0 ? at : -1;
+        if (threadIdx.x < a.per_block && r < a.rows) a.pos_of[r] = t >= 0 ? at : -1;
         if (threadIdx.x == 0) last = base + __popc(mask);
     }
     __syncthreads();
     const int64_t plane = a.rows_pad * a.stride;
     const bool vec = sizeof(T) == 2 && a.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int i = warp; i < kRowsBlock; i += 8)
+    for (int i = warp; i < a.per_block; i += 8)
         if (where[i] >= 0)
-            ce_copy_row(static_cast<const T*>(a.x) + (r0 + i) * a.cols, a.dst + where[i] * a.stride, a.cols, a.stride, plane, vec, lane, 32);
+            ce_copy_row(static_cast<const T*>(a.x) + (r0 + i) * a.cols, a.dst + where[i] * a.stride, a.cols, a.stride, plane, vec, lane);
     if (blockIdx.x + 1 == gridDim.x) {                 // the last block knows the number of rows
         if (threadIdx.x == 0) *a.count = last;
         // rows of dW's sum behind the last one, up to a whole slab
@@ -246,7 +277,27 @@ template <typename T>
 __global__ void __launch_bounds__(256) ce_pack_kernel(const T* w, int64_t rows, int cols, __nv_bfloat16* dst, int64_t rows_pad, int64_t stride) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + warp; r < rows; r += static_cast<int64_t>(gridDim.x) * 8)
-        ce_copy_row(w + r * cols, dst + r * stride, cols, stride, rows_pad * stride, false, lane, 32);
+        ce_copy_row(w + r * cols, dst + r * stride, cols, stride, rows_pad * stride, false, lane);
+}
+
+// ---------------------------------------------------------------- the epilogue's stores
+// A warp's 32 x 32 values (thread = row) go through `stage`; put(row, column, values) gets runs of N columns of a row, N lanes' worth of
+// neighbouring runs per row at a time.
+template <int N, typename F>
+__device__ __forceinline__ void ce_store(float* stage, const float (&v)[32], int lane, F put) {
+    __syncwarp();
+#pragma unroll
+    for (int e = 0; e < 32; ++e) stage[lane * 33 + e] = v[e];
+    __syncwarp();
+    constexpr int per_row = 32 / N;                    // lanes per row; an instruction covers N rows, per_row of them the 32
+#pragma unroll
+    for (int i = 0; i < per_row; ++i) {
+        const int r = lane / per_row + i * N, c = lane % per_row * N;
+        float f[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] = stage[r * 33 + c + e];
+        put(r, c, f);
+    }
 }
 
 // ---------------------------------------------------------------- the products
@@ -259,6 +310,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_con
     __shared__ uint32_t tmem_base;
     __shared__ volatile int abort_flag;
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    __shared__ int hits[8][kHits];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = CG == 1 ? 0 : static_cast<int>(cluster_rank());
     if (threadIdx.x == 0) {
@@ -286,7 +338,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_con
     const int first = blockIdx.x / CG, stride = gridDim.x / CG;
 
     if (warp == 0) {
-        if (lane == 0) {
+        if (elect_one()) {
             const uint32_t full0 = leader_address(&full[0]);
             int fills = 0, s = 0;                      // s: slot of the ring
             uint32_t wrap = 1;                         // parity of the slot's previous use
@@ -344,7 +396,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_con
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0 && elect_one()) {
             int n = 0, s = 0;
             uint32_t phase = 0;
             bool ok = true;
@@ -386,6 +438,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_con
         }
     } else if (warp >= 4) {
         const int quarter = warp & 3, part = (warp - 4) >> 2;     // lanes 32 * quarter.., the part-th half of the columns
+        float* stage = reinterpret_cast<float*>(ring + kStages * R::kStageBytes) + (warp - 4) * kStageFloats;
         const uint32_t acc_empty_at[2] = {leader_address(&acc_empty[0]), leader_address(&acc_empty[1])};
         int n = 0;
         for (int t = first; t < total; t += stride, ++n) {
@@ -394,26 +447,46 @@ __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_con
             const CeShape& sh = j ? s1 : s0;
             const CeTile tile = ce_tile(job, sh, j ? t - s0.tiles : t);
             const int acc = n & 1, width = job.tn >> 1;
+            const int row0 = tile.m0 + rank * kTM + quarter * 32, row = row0 + lane;
+            const bool live = row < sh.m;
+            const int c0 = tile.n0 + part * width;
+            const int c1 = c0 + width < sh.n ? c0 + width : sh.n;          // this thread's columns that exist
+            // dW: the rows whose target is one of this warp's 32 columns of the vocabulary, found while the products run
+            int n_hits = 0;
+            if (job.epi == kEpiDw && a.left_over) {
+                const int base = a.col0 + row0;
+                for (int i0 = 0; i0 < sh.k; i0 += 128) {
+                    int t[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) t[u] = i0 + 32 * u + lane < sh.k ? a.target[i0 + 32 * u + lane] - base : -1;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const bool hit = t[u] >= 0 && t[u] < 32;
+                        const uint32_t mask = __ballot_sync(0xffffffffu, hit);
+                        const int at = n_hits + __popc(mask & ((1u << lane) - 1));
+                        if (hit && at < kHits) hits[warp - 4][at] = (i0 + 32 * u + lane) * 32 + t[u];
+                        n_hits += __popc(mask);
+                    }
+                }
+                __syncwarp();
+            }
             if (!wait_or_abort(&acc_full[acc], (n / 2) & 1, &abort_flag, a.status)) break;
             tc_fence_after();
             const uint32_t d = tmem + acc * kTN + part * width + (static_cast<uint32_t>(quarter * 32) << 16);
-            const int row = tile.m0 + rank * kTM + quarter * 32 + lane;
-            const bool live = row < sh.m;
             const bool empty_sum = tile.iters == 0;    // nothing was multiplied: the accumulators hold something old
-            const int c0 = tile.n0 + part * width;
             if (job.epi == kEpiPairs) {
                 float m = -INFINITY, s = 0.f;
                 const int tgt = live ? a.target[row] - a.col0 : -1;
                 for (int c = c0; c < c0 + width; c += 32) {
                     float v[32];
                     tmem_load32(d + (c - c0), v);
-                    const int left = sh.n - c;
+                    const int left = c1 - c;
                     if (left < 32) {
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
                             if (e >= left) v[e] = -INFINITY;
                     }
-                    if (tgt >= c && tgt < c + 32) {
+                    if (tgt >= c && tgt < c1 && tgt < c + 32) {
                         float zt = 0.f;
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
@@ -422,91 +495,131 @@ __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_con
                     }
                     online_add(v, 1.f, m, s);
                 }
-                if (live) a.pairs[static_cast<int64_t>(a.pair0 + c0 / width) * a.rows_pad + row] = make_float2(m, s);
+                if (live) a.pairs[row * a.n_pairs + a.pair0 + c0 / width] = make_float2(m, s);
             } else if (job.epi == kEpiG) {
                 const int tgt = live ? a.target[row] - a.col0 : -1;
                 const float lse = live ? a.lse[row] : 0.f, gy = live ? a.gy[row] : 0.f;
-                __nv_bfloat16* out = a.g + row * a.g_stride;
+                __nv_bfloat16* out = a.g + row0 * a.g_stride;
                 const int64_t plane = a.rows_pad * a.g_stride;
-                for (int c = c0; c < c0 + width; c += 32) {
+                // columns behind the last one are zeros up to the tile's end: dh and dW read whole slabs of 64
+                const int cz = c0 + width < a.g_stride ? c0 + width : static_cast<int>(a.g_stride);
+                for (int c = c0; c < cz; c += 32) {
                     float v[32];
                     tmem_load32(d + (c - c0), v);
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
                         const float p = ex2f(__fmul_rn(__fsub_rn(v[e], lse), kLog2e));
-                        v[e] = live && c + e < sh.n ? __fmul_rn(gy, tgt == c + e ? __fsub_rn(p, 1.f) : p) : 0.f;
+                        v[e] = live && c + e < c1 ? __fmul_rn(gy, tgt == c + e ? __fsub_rn(p, 1.f) : p) : 0.f;
                     }
-                    if (a.planes == 1) {
+                    if (a.left_over && tgt >= c && tgt < c1 && tgt < c + 32) {
+                        float g = 0.f;
 #pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            *reinterpret_cast<uint4*>(out + c + 8 * q) = Unit<__nv_bfloat16, 16>::pack(v + 8 * q);
-                    } else {
+                        for (int e = 0; e < 32; ++e)
+                            if (tgt == c + e) g = v[e];
+                        a.left_over[row] = __fsub_rn(g, __bfloat162float(__float2bfloat16_rn(g)));
+                    }
+                    ce_store<8>(stage, v, lane, [&](int r, int cc, const float (&f)[8]) {
+                        if (c + cc >= cz) return;
+                        __nv_bfloat16* o = out + r * a.g_stride + c + cc;
+                        if (a.planes == 1) {
+                            *reinterpret_cast<uint4*>(o) = Unit<__nv_bfloat16, 16>::pack(f);
+                        } else {
+                            uint32_t p0[4], p1[4], p2[4];
 #pragma unroll
-                        for (int q = 0; q < 16; ++q) {
-                            uint32_t h0, m0, l0, h1, m1, l1;
-                            split3(v[2 * q], h0, m0, l0);
-                            split3(v[2 * q + 1], h1, m1, l1);
-                            *reinterpret_cast<uint32_t*>(out + c + 2 * q) = (h0 >> 16) | h1;
-                            *reinterpret_cast<uint32_t*>(out + plane + c + 2 * q) = (m0 >> 16) | m1;
-                            *reinterpret_cast<uint32_t*>(out + 2 * plane + c + 2 * q) = (l0 >> 16) | l1;
+                            for (int q = 0; q < 4; ++q) {
+                                uint32_t h0, m0, l0, h1, m1, l1;
+                                split3(f[2 * q], h0, m0, l0);
+                                split3(f[2 * q + 1], h1, m1, l1);
+                                p0[q] = (h0 >> 16) | h1;
+                                p1[q] = (m0 >> 16) | m1;
+                                p2[q] = (l0 >> 16) | l1;
+                            }
+                            *reinterpret_cast<uint4*>(o) = make_uint4(p0[0], p0[1], p0[2], p0[3]);
+                            *reinterpret_cast<uint4*>(o + plane) = make_uint4(p1[0], p1[1], p1[2], p1[3]);
+                            *reinterpret_cast<uint4*>(o + 2 * plane) = make_uint4(p2[0], p2[1], p2[2], p2[3]);
                         }
-                    }
+                    });
                 }
             } else if (job.epi == kEpiDh) {
-                float* out = a.dh + (static_cast<int64_t>(tile.split) * a.rows_pad + row) * a.dh_stride;
-                for (int c = c0; c < c0 + width && c < sh.n; c += 32) {
+                float* out = a.dh + (static_cast<int64_t>(tile.split) * a.rows_pad + row0) * a.dh_stride;
+                for (int c = c0; c < c1; c += 32) {
                     float v[32];
                     tmem_load32(d + (c - c0), v);
-                    if (!live) continue;
-#pragma unroll
-                    for (int q = 0; q < 8; ++q) {
-                        if (c + 4 * q >= a.dh_stride) break;          // the stride is the width rounded up to 4
-                        float4* o = reinterpret_cast<float4*>(out + c + 4 * q);
-                        float4 w = empty_sum ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                    ce_store<4>(stage, v, lane, [&](int r, int cc, const float (&f)[4]) {
+                        if (row0 + r >= sh.m || c + cc >= c1) return;         // the stride is the width rounded up to 4
+                        float4* o = reinterpret_cast<float4*>(out + r * a.dh_stride + c + cc);
+                        float4 w = empty_sum ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(f[0], f[1], f[2], f[3]);
                         if (a.dh_add) {
                             const float4 old = *o;
                             w = make_float4(__fadd_rn(old.x, w.x), __fadd_rn(old.y, w.y), __fadd_rn(old.z, w.z), __fadd_rn(old.w, w.w));
                         }
                         *o = w;
-                    }
+                    });
                 }
             } else {
-                const int64_t at = static_cast<int64_t>(a.col0 + row) * a.hidden;
+                const int64_t at = static_cast<int64_t>(a.col0 + row0) * a.hidden;
                 const bool vec = a.hidden % 8 == 0 && (reinterpret_cast<uintptr_t>(a.dw) & 15) == 0;
-                for (int c = c0; c < c0 + width && c < sh.n; c += 32) {
+                for (int c = c0; c < c1; c += 32) {
                     float v[32];
                     tmem_load32(d + (c - c0), v);
-                    if (!live) continue;
                     if (empty_sum) {
 #pragma unroll
                         for (int e = 0; e < 32; ++e) v[e] = 0.f;
                     }
-                    if (a.dw_f32) {
-                        float* o = static_cast<float*>(a.dw) + at + c;
+                    auto add_left_over = [&](int i) {
+                        const float left = a.left_over[i];
+                        const uint4* h = reinterpret_cast<const uint4*>(a.h + i * a.h_stride + c);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (c + e < sh.n) {
-                                if (a.dw_add) v[e] = __fadd_rn(v[e], o[e]);
-                                if (!vec) o[e] = v[e];
+                        for (int q = 0; q < 4; ++q)
+                            if (c + 8 * q < c1) {
+                                float f[8];
+                                Unit<__nv_bfloat16, 16>::unpack(h[q], f);
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) v[8 * q + e] = __fmaf_rn(left, f[e], v[8 * q + e]);
                             }
-                        if (vec) {
-#pragma unroll
-                            for (int q = 0; q < 8; ++q)
-                                if (c + 4 * q < sh.n) reinterpret_cast<float4*>(o)[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                    };
+                    if (n_hits <= kHits) {
+                        for (int k = 0; k < n_hits; ++k) {
+                            const int x = hits[warp - 4][k];
+                            if ((x & 31) == lane) add_left_over(x >> 5);
                         }
+                    } else {                           // more than the list holds: all targets once more, in the same order
+                        for (int i = 0; i < sh.k; ++i)
+                            if (a.target[i] - a.col0 == row) add_left_over(i);
+                    }
+                    if (!vec) {
+                        ce_store<1>(stage, v, lane, [&](int r, int cc, const float (&f)[1]) {
+                            if (row0 + r >= sh.m || c + cc >= c1) return;
+                            const int64_t o = at + static_cast<int64_t>(r) * a.hidden + c + cc;
+                            if (a.dw_f32) {
+                                float* w = static_cast<float*>(a.dw) + o;
+                                *w = a.dw_add ? __fadd_rn(f[0], *w) : f[0];
+                            } else {
+                                __nv_bfloat16* w = static_cast<__nv_bfloat16*>(a.dw) + o;
+                                *w = __float2bfloat16_rn(a.dw_add ? __fadd_rn(f[0], __bfloat162float(*w)) : f[0]);
+                            }
+                        });
+                    } else if (a.dw_f32) {
+                        ce_store<4>(stage, v, lane, [&](int r, int cc, const float (&f)[4]) {
+                            if (row0 + r >= sh.m || c + cc >= c1) return;
+                            float4* o = reinterpret_cast<float4*>(static_cast<float*>(a.dw) + at + static_cast<int64_t>(r) * a.hidden + c + cc);
+                            float4 w = make_float4(f[0], f[1], f[2], f[3]);
+                            if (a.dw_add) {
+                                const float4 old = *o;
+                                w = make_float4(__fadd_rn(old.x, w.x), __fadd_rn(old.y, w.y), __fadd_rn(old.z, w.z), __fadd_rn(old.w, w.w));
+                            }
+                            __stcs(o, w);
+                        });
                     } else {
-                        __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.dw) + at + c;
+                        ce_store<8>(stage, v, lane, [&](int r, int cc, const float (&f)[8]) {
+                            if (row0 + r >= sh.m || c + cc >= c1) return;
+                            uint4* o = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.dw) + at + static_cast<int64_t>(r) * a.hidden + c + cc);
+                            float w[8];
+                            if (a.dw_add) Unit<__nv_bfloat16, 16>::unpack(*o, w);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (c + e < sh.n) {
-                                if (a.dw_add) v[e] = __fadd_rn(v[e], __bfloat162float(o[e]));
-                                if (!vec) o[e] = __float2bfloat16_rn(v[e]);
-                            }
-                        if (vec) {
-#pragma unroll
-                            for (int q = 0; q < 4; ++q)
-                                if (c + 8 * q < sh.n) reinterpret_cast<uint4*>(o)[q] = Unit<__nv_bfloat16, 16>::pack(v + 8 * q);
-                        }
+                            for (int e = 0; e < 8; ++e) w[e] = a.dw_add ? __fadd_rn(f[e], w[e]) : f[e];
+                            store_vec_streaming(o, Unit<__nv_bfloat16, 16>::pack(w));
+                        });
                     }
                 }
             }
@@ -527,39 +640,94 @@ __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_con
 }
 
 // ---------------------------------------------------------------- joining
-// lse and loss of the rows that take part, from their pairs.  blockDim (32, 8): 32 rows, eight runs of pairs.
-__global__ void __launch_bounds__(256) ce_join_kernel(const float2* pairs, int n, int64_t rows_pad, const int* count, const float* z_target,
-                                                      const int* row_of, float* loss, float* lse) {
-    __shared__ float2 part[8][33];
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x;
-    const bool live = i < *count;
-    float m = -INFINITY, s = 0.f;
-    if (live)
-        for (int p = threadIdx.y; p < n; p += 8) {
-            const float2 q = pairs[p * rows_pad + i];
-            join_pair(m, s, q.x, q.y);
-        }
-    part[threadIdx.y][threadIdx.x] = make_float2(m, s);
-    __syncthreads();
-    if (threadIdx.y || !live) return;
-    for (int p = 1; p < 8; ++p) join_pair(m, s, part[p][threadIdx.x].x, part[p][threadIdx.x].y);
-    const float l = __fadd_rn(m, logf(s));
+// lse and loss of the rows that take part, a warp per row.  The loss is a difference of two numbers of the size of the logits, and the
+// tensor cores cut (not round) every partial sum: z_target there was off by 1.5e-5 at 4096 terms of one sign.  So z_target is computed
+// once more, in fp32, and takes its own place in the sum of exponentials as well: the two agree, and the loss of a target with p near one
+// is not a difference of two errors.
+template <typename T>
+__global__ void __launch_bounds__(256) ce_join_kernel(const float2* pairs, int n, int64_t n_pairs, const int* count, const float* z_target,
+                                                      const int* target_of, const int* row_of, const T* h, const T* w, int hidden, float* loss,
+                                                      float* lse) {
+    const int i = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (i >= *count) return;
     const int r = row_of[i];
+    const T* hr = h + static_cast<int64_t>(r) * hidden;
+    const T* wr = w + static_cast<int64_t>(target_of[i]) * hidden;
+    typedef Unit<T, 16> U;
+    float z = 0.f;
+    if (hidden % U::N == 0 && ((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(w)) & 15) == 0) {
+        const uint4* hv = reinterpret_cast<const uint4*>(hr);
+        const uint4* wv = reinterpret_cast<const uint4*>(wr);
+#pragma unroll 4
+        for (int c = lane; c < hidden / U::N; c += 32) {
+            float f[U::N], g[U::N];
+            U::unpack(hv[c], f);
+            U::unpack(wv[c], g);
+#pragma unroll
+            for (int e = 0; e < U::N; ++e) z = __fmaf_rn(f[e], g[e], z);
+        }
+    } else {
+#pragma unroll 8
+        for (int c = lane; c < hidden; c += 32) z = __fmaf_rn(Vec<T>::load1(hr + c), Vec<T>::load1(wr + c), z);
+    }
+    float m = -INFINITY, s = 0.f;
+#pragma unroll 4
+    for (int p = lane; p < n; p += 32) {
+        const float2 q = pairs[i * n_pairs + p];
+        join_pair(m, s, q.x, q.y);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        z = __fadd_rn(z, __shfl_xor_sync(0xffffffffu, z, o));
+        const float mb = __shfl_xor_sync(0xffffffffu, m, o), sb = __shfl_xor_sync(0xffffffffu, s, o);
+        join_pair(m, s, mb, sb);
+    }
+    if (lane) return;
+    s = __fadd_rn(s, __fsub_rn(exp2f(__fmul_rn(__fsub_rn(z, m), kLog2e)), exp2f(__fmul_rn(__fsub_rn(z_target[i], m), kLog2e))));
+    const float l = __fadd_rn(m, logf(s));
     lse[r] = l;
-    loss[r] = __fsub_rn(l, z_target[i]);
+    loss[r] = __fsub_rn(l, z);
 }
 
-// dh of every row: the parts summed in order and rounded once, zeros where the row took no part.
+// dh of every row: the parts summed in order, what rounding took from g at the target times that row of W, rounded once; zeros where
+// the row took no part.  A thread takes four neighbouring columns.
 template <typename T>
-__global__ void __launch_bounds__(256) ce_dh_kernel(const float* parts, int splits, int64_t rows_pad, int64_t stride, const int* pos_of, T* dh,
-                                                    int64_t rows, int hidden) {
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+__global__ void __launch_bounds__(256) ce_dh_kernel(const float* parts, int splits, int64_t rows_pad, int64_t stride, const int* pos_of,
+                                                    const int* target_of, const float* left_over, const T* w, T* dh, int64_t rows, int hidden) {
+    const int quads = (hidden + 3) / 4;
+    const bool vec = sizeof(T) == 4 ? hidden % 4 == 0 && (reinterpret_cast<uintptr_t>(dh) & 15) == 0
+                                    : hidden % 4 == 0 && (reinterpret_cast<uintptr_t>(dh) & 7) == 0;
+    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
         const int p = pos_of[r];
-        for (int c = threadIdx.x; c < hidden; c += 256) {
-            float s = 0.f;
-            if (p >= 0)
-                for (int k = 0; k < splits; ++k) s = __fadd_rn(s, parts[(static_cast<int64_t>(k) * rows_pad + p) * stride + c]);
-            Vec<T>::store1(dh + r * hidden + c, s);
+        const T* wr = p >= 0 && left_over ? w + static_cast<int64_t>(target_of[p]) * hidden : nullptr;
+        const float left = wr ? left_over[p] : 0.f;
+        for (int q = blockIdx.x * 256 + threadIdx.x; q < quads; q += gridDim.x * 256) {
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
+            if (p >= 0) {
+#pragma unroll 4
+                for (int k = 0; k < splits; ++k) {
+                    const float4 v = *reinterpret_cast<const float4*>(parts + (k * rows_pad + p) * stride + 4 * q);
+                    s[0] = __fadd_rn(s[0], v.x);
+                    s[1] = __fadd_rn(s[1], v.y);
+                    s[2] = __fadd_rn(s[2], v.z);
+                    s[3] = __fadd_rn(s[3], v.w);
+                }
+                if (wr) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (4 * q + e < hidden) s[e] = __fmaf_rn(left, Vec<T>::load1(wr + 4 * q + e), s[e]);
+                }
+            }
+            T* o = dh + r * hidden + 4 * q;
+            if (vec && sizeof(T) == 4) {
+                *reinterpret_cast<float4*>(o) = make_float4(s[0], s[1], s[2], s[3]);
+            } else if (vec) {
+                *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3]));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (4 * q + e < hidden) Vec<T>::store1(o + e, s[e]);
+            }
         }
     }
 }

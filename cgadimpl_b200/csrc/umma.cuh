@@ -8,15 +8,34 @@
 namespace agb {
 
 // ---------------------------------------------------------------- waits
-// A wait that gives up after kWaitPollLimit polls, or as soon as another role of the CTA has given up.
+// A wait that gives up after kTcPollLimit polls, or as soon as another role of the CTA has given up.  The polls carry no time
+// hint: with the 10 us hint of mbar_try_wait the 4096 x 4096 x 18944 loss took 423 us, without it 413 us.  A poll takes 20 ns at
+// least, so the limit is 80 ms or more, against the few milliseconds of the longest tile.
+constexpr int kTcPollLimit = 1 << 22;
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status) {
-    for (int i = 0; i < kWaitPollLimit; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
+    for (int i = 0; i < kTcPollLimit; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+        if (ok) return true;
         if (*abort_flag) return false;
     }
     *abort_flag = 1;
     atomicExch(status, 6 /* AGB_ERR_TIMEOUT */);
     return false;
+}
+// One lane of the warp.  The branches that issue TMA and tcgen05 instructions are taken by elect.sync, not by comparing the lane
+// number: those instructions want warp-uniform operands, and where the compiler sees that one lane alone runs the branch it needs no
+// loop over lanes around each of them (4096 x 4096 x 18944 loss: 511 us with `lane == 0`, 423 us with this).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p != 0;
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
