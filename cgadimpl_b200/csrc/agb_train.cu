@@ -192,15 +192,17 @@ EncodeTiled encode_tiled() {
     }();
     return f;
 }
-// A [planes][rows][cols] bf16 tensor with rows `stride` elements apart, read in boxes of 64 columns by `box_rows` rows.
-int make_map(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int planes, int64_t stride, int64_t plane, int box_rows) {
+// A [planes][rows][cols] tensor (bf16, or fp32) with rows `stride` elements apart, in boxes of 128 bytes by `box_rows` rows.
+int make_map(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int planes, int64_t stride, int64_t plane, int box_rows,
+             bool f32 = false) {
+    const int elem = f32 ? 4 : 2;
     EncodeTiled f = encode_tiled();
     if (!f) return fail(AGB_ERR_CUDA, "cuTensorMapEncodeTiled is not available in this driver");
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(planes)};
-    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(stride) * 2, static_cast<cuuint64_t>(plane) * 2};
-    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_rows), 1};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(stride) * elem, static_cast<cuuint64_t>(plane) * elem};
+    const cuuint32_t box[3] = {static_cast<cuuint32_t>(128 / elem), static_cast<cuuint32_t>(box_rows), 1};
     const cuuint32_t steps[3] = {1, 1, 1};
-    const CUresult r = f(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, steps,
+    const CUresult r = f(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, steps,
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(AGB_ERR_CUDA, "cuTensorMapEncodeTiled: error %d", static_cast<int>(r));
@@ -214,12 +216,13 @@ constexpr int64_t kCeGLimit = 256LL << 20;      // bytes of g at once
 struct CePlan {
     int planes;
     bool direct_w;              // TMA reads W as it is
+    bool direct_dw;             // and writes dW as it is
     int64_t rows_pad, k_stride, piece, pieces, g_stride, dh_stride, pairs;
     int pair;                   // CTAs that work on a tile together
     int tn;                     // columns of a tile of logits
     int64_t pairs_per_piece;
     int splits, k_per_split;
-    size_t h, w, count, row_of, pos_of, target_of, lse_of, gy_of, left_over, z_target, pair_at, g, dh, total;
+    size_t h, w, count, row_of, pos_of, target_of, lse_of, gy_of, gy_scale, left_over, z_target, pair_at, g, dh, dw, total;
 };
 
 // Columns of a tile of logits.  A slab of a tile takes the longest of its products (2 clocks per column), its bytes from L2 at 64 a
@@ -229,7 +232,7 @@ int choose_tn(int pair, int64_t rows, int64_t columns, int step, int sms) {
     const int64_t mt = ceil_div(rows, pair * agb::kTM), units = sms / pair;
     int best = 256;
     double least = 0;
-    for (int tn = 256; tn >= 64; tn -= step) {
+    for (int tn = 256; tn >= (step < 64 ? 64 : step); tn -= step) {
         double slab = 2.0 * tn;
         const double l2 = (agb::kTM * 128 + tn / pair * 128) / 64.0, dram = tn / pair * 128 / 24.0 / static_cast<double>(mt);
         if (l2 > slab) slab = l2;
@@ -247,6 +250,7 @@ CePlan plan_ce(bool backward, int64_t rows, int64_t hidden, int64_t vocab, int d
     CePlan p{};
     p.planes = dtype == AGB_F32 ? 3 : 1;
     p.direct_w = dtype == AGB_BF16 && hidden % 8 == 0;
+    p.direct_dw = hidden % (dtype == AGB_BF16 ? 8 : 4) == 0;
     p.rows_pad = ceil_div(rows, 2 * agb::kTM) * 2 * agb::kTM;
     p.k_stride = ceil_div(hidden, 8) * 8;
     p.piece = ceil_div(vocab, 256) * 256;
@@ -263,7 +267,7 @@ CePlan plan_ce(bool backward, int64_t rows, int64_t hidden, int64_t vocab, int d
     p.g_stride = p.piece;
     p.dh_stride = ceil_div(hidden, 4) * 4;
     p.pair = rows <= agb::kTM ? 1 : 2;     // rows that fit one CTA's half of a pair's tile leave nothing for the other to do
-    p.tn = choose_tn(p.pair, rows, p.piece < vocab ? p.piece : vocab, backward ? 64 : 32, sms);
+    p.tn = choose_tn(p.pair, rows, p.piece < vocab ? p.piece : vocab, backward ? 128 : 32, sms);
     p.pairs_per_piece = ceil_div(p.piece, p.tn) * 2;
     p.pairs = p.pieces * p.pairs_per_piece;
     // dh: few tiles with a long sum are cut along it, until the GPU has two per SM or a part has 16 slabs
@@ -288,7 +292,9 @@ CePlan plan_ce(bool backward, int64_t rows, int64_t hidden, int64_t vocab, int d
         take(&p.lse_of, p.rows_pad * 4);
         take(&p.gy_of, p.rows_pad * 4);
         take(&p.left_over, p.rows_pad * 4);
+        take(&p.gy_scale, 4);
         take(&p.g, static_cast<size_t>(p.planes) * p.rows_pad * p.g_stride * 2);
+        if (!p.direct_dw) take(&p.dw, static_cast<size_t>(p.piece) * p.k_stride * 4);
         if (want_dh) take(&p.dh, static_cast<size_t>(p.splits) * p.rows_pad * p.dh_stride * 4);
     } else {
         take(&p.z_target, p.rows_pad * 4);
@@ -343,6 +349,7 @@ int ce_rows(const CeCall& c, const float* lse, const float* gy, float* loss, flo
     if (lse) {
         a.lse_of = c.at<float>(c.p.lse_of);
         a.gy_of = c.at<float>(c.p.gy_of);
+        a.gy_scale = c.at<float>(c.p.gy_scale);
     }
     a.loss = loss;
     a.lse_out = lse_out;
@@ -364,6 +371,19 @@ int ce_pack(const CeCall& c, int64_t col0, int64_t n) {
         agb::ce_pack_kernel<bf16><<<static_cast<unsigned>(grid), 256, 0, c.st>>>(static_cast<const bf16*>(c.w) + col0 * c.hidden, n, (int)c.hidden,
                                                                                 c.at<bf16>(c.p.w), c.p.piece, c.p.k_stride);
     return after_launch("linear_ce_pack");
+}
+int ce_unpack(const CeCall& c, void* dw, int64_t col0, int64_t n, bool f32, int add) {
+    int64_t grid = ceil_div(n, 8);
+    if (grid > 16LL * c.d.sms) grid = 16LL * c.d.sms;
+    const unsigned g = static_cast<unsigned>(grid);
+    const int cols = static_cast<int>(c.hidden);
+    if (c.dtype == AGB_F32)
+        agb::ce_unpack_kernel<float, float><<<g, 256, 0, c.st>>>(c.at<float>(c.p.dw), n, cols, c.p.k_stride, static_cast<float*>(dw) + col0 * c.hidden, add);
+    else if (f32)
+        agb::ce_unpack_kernel<float, bf16><<<g, 256, 0, c.st>>>(c.at<float>(c.p.dw), n, cols, c.p.k_stride, static_cast<bf16*>(dw) + col0 * c.hidden, add);
+    else
+        agb::ce_unpack_kernel<bf16, bf16><<<g, 256, 0, c.st>>>(c.at<bf16>(c.p.dw), n, cols, c.p.k_stride, static_cast<bf16*>(dw) + col0 * c.hidden, add);
+    return after_launch("linear_ce_unpack");
 }
 // W, or its piece where it was laid out: rows of the map, and the map's row of the piece's first column.
 int map_w(const CeCall& c, CUtensorMap* m, int64_t n, int box_rows) {
@@ -402,7 +422,7 @@ agb::CeJob logits_job(const CeCall& c, int epi, int64_t col0, int64_t n) {
     j.b_box = j.tn / c.p.pair;
     return j;
 }
-template <int CG>
+template <int CG, int PHASE>
 int launch_gemm_cg(const CeCall& c, const agb::CeArgs& a) {
     int64_t tiles = 0;
     for (int i = 0; i < a.jobs; ++i) {
@@ -410,12 +430,12 @@ int launch_gemm_cg(const CeCall& c, const agb::CeArgs& a) {
         tiles += ceil_div(j.m < 0 ? c.rows : j.m, CG * agb::kTM) * ceil_div(j.n, j.tn) * j.splits;
     }
     if (tiles >= (1LL << 31)) return fail(AGB_ERR_UNSUPPORTED, "too many tiles");
-    AGB_CUDA(cudaFuncSetAttribute(agb::ce_gemm_kernel<CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, agb::CeRing<CG>::kSmem));
+    AGB_CUDA(cudaFuncSetAttribute(agb::ce_gemm_kernel<CG, PHASE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (agb::CeRing<CG, PHASE>::kSmem)));
     const int64_t most = c.d.sms / CG;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>((tiles < most ? tiles : most) * CG));
     cfg.blockDim = dim3(agb::kCeThreads);
-    cfg.dynamicSmemBytes = agb::CeRing<CG>::kSmem;
+    cfg.dynamicSmemBytes = (agb::CeRing<CG, PHASE>::kSmem);
     cfg.stream = c.st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -424,11 +444,12 @@ int launch_gemm_cg(const CeCall& c, const agb::CeArgs& a) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    AGB_CUDA(cudaLaunchKernelEx(&cfg, agb::ce_gemm_kernel<CG>, a));
+    AGB_CUDA(cudaLaunchKernelEx(&cfg, agb::ce_gemm_kernel<CG, PHASE>, a));
     return after_launch("linear_ce_gemm");
 }
+template <int PHASE>
 int launch_gemm(const CeCall& c, const agb::CeArgs& a) {
-    return c.p.pair == 1 ? launch_gemm_cg<1>(c, a) : launch_gemm_cg<2>(c, a);
+    return c.p.pair == 1 ? launch_gemm_cg<1, PHASE>(c, a) : launch_gemm_cg<2, PHASE>(c, a);
 }
 
 int start_ce(CeCall* c, bool backward, bool want_dh, void* workspace, size_t workspace_bytes, agb_stream_t stream) {
@@ -480,7 +501,7 @@ int agb_linear_ce_fwd(const void* h, const void* w, const void* target, int targ
         a.col0 = static_cast<int>(col0);
         a.n_pairs = c.p.pairs;
         a.pair0 = static_cast<int>(i * c.p.pairs_per_piece);
-        AGB_TRY(launch_gemm(c, a));
+        AGB_TRY(launch_gemm<0>(c, a));
     }
     const int64_t last = vocab - (c.p.pieces - 1) * c.p.piece;
     const int pairs = static_cast<int>((c.p.pieces - 1) * c.p.pairs_per_piece + ceil_div(last, c.p.tn) * 2);
@@ -529,9 +550,9 @@ int agb_linear_ce_bwd(const void* h, const void* w, const void* target, int targ
         a.g = c.at<bf16>(c.p.g);
         a.g_stride = c.p.g_stride;
         a.left_over = c.p.planes == 1 ? c.at<float>(c.p.left_over) : nullptr;
-        a.h = c.at<bf16>(c.p.h);
-        a.h_stride = c.p.k_stride;
-        AGB_TRY(launch_gemm(c, a));
+        a.gy_scale = c.at<float>(c.p.gy_scale);
+        AGB_TRY(map_g(c, &a.out[0], 32));
+        AGB_TRY(c.p.planes == 1 ? launch_gemm<1>(c, a) : launch_gemm<3>(c, a));
         a.jobs = 0;
         if (dh) {
             agb::CeJob& j = a.job[a.jobs];
@@ -553,6 +574,7 @@ int agb_linear_ce_bwd(const void* h, const void* w, const void* target, int targ
             a.dh = c.at<float>(c.p.dh);
             a.dh_stride = c.p.dh_stride;
             a.dh_add = i > 0;
+            AGB_TRY(make_map(&a.out[a.jobs], a.dh, c.p.dh_stride, c.p.rows_pad, c.p.splits, c.p.dh_stride, c.p.rows_pad * c.p.dh_stride, 32, true));
             ++a.jobs;
         }
         if (dw) {
@@ -574,20 +596,31 @@ int agb_linear_ce_bwd(const void* h, const void* w, const void* target, int targ
             a.dw = dw;
             a.dw_add = accumulate_dw != 0;
             a.dw_f32 = dtype == AGB_F32;
+            if (!c.p.direct_dw) {
+                a.dw_out = agb::kDwStaged;
+                a.dw_f32 = a.dw_f32 || a.dw_add;
+                AGB_TRY(make_map(&a.out[a.jobs], c.at<void>(c.p.dw), c.p.k_stride, n, 1, c.p.k_stride, c.p.piece * c.p.k_stride, 32, a.dw_f32));
+            } else if (addr(dw) % 16 == 0) {
+                a.dw_out = agb::kDwTma;
+                AGB_TRY(make_map(&a.out[a.jobs], dw, hidden, vocab, 1, hidden, vocab * hidden, 32, a.dw_f32));
+            } else {
+                a.dw_out = agb::kDwScalar;
+            }
             ++a.jobs;
         }
-        AGB_TRY(launch_gemm(c, a));
+        AGB_TRY(launch_gemm<2>(c, a));
+        if (dw && a.dw_out == agb::kDwStaged) AGB_TRY(ce_unpack(c, dw, col0, n, a.dw_f32, accumulate_dw));
     }
     if (dh) {
         const dim3 grid(static_cast<unsigned>(ceil_div(ceil_div(hidden, 4), 256)), static_cast<unsigned>(rows < 32768 ? rows : 32768));
         const float* left = c.p.planes == 1 ? c.at<float>(c.p.left_over) : nullptr;
         if (dtype == AGB_F32)
             agb::ce_dh_kernel<float><<<grid, 256, 0, c.st>>>(c.at<float>(c.p.dh), c.p.splits, c.p.rows_pad, c.p.dh_stride, c.at<int>(c.p.pos_of),
-                                                             c.at<int>(c.p.target_of), left, static_cast<const float*>(w), static_cast<float*>(dh),
+                                                             c.at<int>(c.p.target_of), left, c.at<float>(c.p.gy_scale), static_cast<const float*>(w), static_cast<float*>(dh),
                                                              rows, (int)hidden);
         else
             agb::ce_dh_kernel<bf16><<<grid, 256, 0, c.st>>>(c.at<float>(c.p.dh), c.p.splits, c.p.rows_pad, c.p.dh_stride, c.at<int>(c.p.pos_of),
-                                                            c.at<int>(c.p.target_of), left, static_cast<const bf16*>(w), static_cast<bf16*>(dh),
+                                                            c.at<int>(c.p.target_of), left, c.at<float>(c.p.gy_scale), static_cast<const bf16*>(w), static_cast<bf16*>(dh),
                                                             rows, (int)hidden);
         return after_launch("linear_ce_dh");
     }

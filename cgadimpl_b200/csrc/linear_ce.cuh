@@ -25,16 +25,15 @@ constexpr int kTM = 128, kTN = 256, kTK = 64;          // rows of A per CTA, mos
 constexpr int kCeThreads = 384;        // TMA, MMA, TMEM, idle, and eight warps of epilogue
 // CG CTAs work on a tile of CG * 128 rows together (tcgen05 cta_group): each holds its 128 rows of A, its share of the columns of
 // B and the accumulators of its rows.  A pair reads half of B per CTA, so its ring is deeper for the same bytes.
-// Behind the ring each epilogue warp has 32 x 32 floats (rows 33 apart) through which a thread's run of columns becomes a row's: stores
-// of 64 bytes and more per row instead of 32 rows touched by each instruction.
-constexpr int kStageFloats = 32 * 33;
-constexpr int kHits = 16;
-template <int CG>
+// Behind the ring each epilogue warp has boxes of 4 KB (32 rows of 128 bytes) in which its results leave by TMA, in turn.
+constexpr int kBoxBytes = 32 * 128;
+template <int CG, int PHASE>
 struct CeRing {
     static constexpr int kStages = CG == 1 ? 4 : 6;
+    static constexpr int kBoxes = PHASE == 0 ? 0 : 1;
     static constexpr int kBytesA = kTM * kTK * 2, kBytesB = kTN / CG * kTK * 2;
     static constexpr int kStageBytes = kBytesA + kBytesB;
-    static constexpr int kSmem = kStages * kStageBytes + 8 * kStageFloats * 4 + 1024;
+    static constexpr int kSmem = kStages * kStageBytes + 8 * kBoxes * kBoxBytes + 1024;
 };
 
 // What an epilogue does with its tile.
@@ -52,8 +51,13 @@ struct CeJob {
 };
 constexpr int kMGroup = 4096;
 
+// dw leaves by TMA to its place; or, where its rows are no multiple of 16 bytes, to a buffer with rows that are (in 32 bits if it is to be
+// added), from which ce_unpack_kernel takes it; or, where only its base lies between, element by element.
+enum CeDw { kDwTma = 0, kDwStaged = 1, kDwScalar = 2 };
+
 struct CeArgs {
     CUtensorMap A[2], B[2];
+    CUtensorMap out[2];                // of the job's results, boxes of 32 rows of 128 bytes
     CeJob job[2];
     int jobs;
     const int* count;                  // rows that take part
@@ -70,6 +74,7 @@ struct CeArgs {
     const float *lse, *gy;             // [rows_pad]
     __nv_bfloat16* g;                  // [planes][rows_pad][g_stride]
     float* left_over;                  // [rows_pad]: what rounding took from g at the row's target (one plane only, else NULL)
+    const float* gy_scale;             // the largest |gy|: g is kept relative to it
     int64_t g_stride;
     int planes;
     // dh: fp32 parts [split][rows_pad][dh_stride]
@@ -78,9 +83,8 @@ struct CeArgs {
     int dh_add;                        // 0 the first piece: write, 1 add
     // dw
     void* dw;
-    const __nv_bfloat16* h;            // [rows_pad][h_stride], for what is left over
-    int64_t h_stride;
     int hidden, dw_add, dw_f32;
+    int dw_out;                        // how dw leaves: CeDw
 };
 
 struct CeTile {
@@ -162,7 +166,7 @@ struct CeRowsArgs {
     int* pos_of;                       // [rows]: where the row went, or -1
     int* target_of;                    // [rows_pad]
     const float *lse, *gy;             // backward: [rows]; NULL in the forward
-    float *lse_of, *gy_of;
+    float *lse_of, *gy_of, *gy_scale;
     float *loss, *lse_out;             // forward: rows that take no part get 0
 };
 constexpr int kRowsBlock = 32;         // most rows of a block
@@ -225,6 +229,7 @@ __global__ void __launch_bounds__(256) ce_rows_kernel(const CeRowsArgs a) {
     __shared__ int warp_count[8];
     __shared__ int where[kRowsBlock];
     __shared__ int last;
+    __shared__ float scale_of[8];
     const int64_t r0 = static_cast<int64_t>(blockIdx.x) * a.per_block;
     int n = 0;
 #pragma unroll 4
@@ -263,6 +268,19 @@ __global__ void __launch_bounds__(256) ce_rows_kernel(const CeRowsArgs a) {
             ce_copy_row(static_cast<const T*>(a.x) + (r0 + i) * a.cols, a.dst + where[i] * a.stride, a.cols, a.stride, plane, vec, lane);
     if (blockIdx.x + 1 == gridDim.x) {                 // the last block knows the number of rows
         if (threadIdx.x == 0) *a.count = last;
+        if (a.lse) {                                   // the largest |gy| of the rows that take part, 1 where that is no scale
+            float top = 0.f;
+#pragma unroll 4
+            for (int64_t r = threadIdx.x; r < a.rows; r += 256)
+                if (ce_target(a, r) >= 0) top = fmaxf(top, fabsf(a.gy[r]));
+            top = warp_max(top);
+            if (lane == 0) scale_of[warp] = top;
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                for (int w = 1; w < 8; ++w) top = fmaxf(top, scale_of[w]);
+                *a.gy_scale = top > 0x1p-100f && top < 0x1p100f ? top : 1.f;
+            }
+        }
         // rows of dW's sum behind the last one, up to a whole slab
         const int64_t stop = (static_cast<int64_t>(last) + kTK - 1) / kTK * kTK;
         for (int p = 0; a.lse && p < a.planes; ++p) {
@@ -281,36 +299,74 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const T* w, int64_t rows, 
 }
 
 // ---------------------------------------------------------------- the epilogue's stores
-// A warp's 32 x 32 values (thread = row) go through `stage`; put(row, column, values) gets runs of N columns of a row, N lanes' worth of
-// neighbouring runs per row at a time.
-template <int N, typename F>
-__device__ __forceinline__ void ce_store(float* stage, const float (&v)[32], int lane, F put) {
+// Eight 16-byte words of a row (thread = row) into the next swizzled box, then one lane sends it off: send(box).
+template <int BOXES, typename F>
+__device__ __forceinline__ void ce_send(uint8_t* boxes, int& turn, const uint4 (&w)[8], int lane, F send) {
+    tma_store_wait_read<BOXES - 1>();                  // the lane that sent this box last: it has been read
     __syncwarp();
+    uint8_t* box = boxes + turn * kBoxBytes;
+    if (++turn == BOXES) turn = 0;
 #pragma unroll
-    for (int e = 0; e < 32; ++e) stage[lane * 33 + e] = v[e];
+    for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(box + lane * 128 + ((q ^ (lane & 7)) << 4)) = w[q];
+    fence_async();
     __syncwarp();
-    constexpr int per_row = 32 / N;                    // lanes per row; an instruction covers N rows, per_row of them the 32
+    if (lane == 0) {
+        send(box);
+        tma_store_commit();
+    }
+}
+
+// A staged piece of dw [rows][stride] (S: bf16, or fp32 that is still to be rounded or added) to its place [rows][cols].  A warp per row;
+// 16-bit rows that start between two words are written as a single element and pairs.
+template <typename S, typename T>
+__global__ void __launch_bounds__(256) ce_unpack_kernel(const S* src, int64_t rows, int cols, int64_t stride, T* dw, int add) {
+    constexpr int B = 8;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + warp; r < rows; r += static_cast<int64_t>(gridDim.x) * 8) {
+        const S* s = src + r * stride;
+        T* d = dw + r * cols;
+        const int odd = sizeof(T) == 2 && (reinterpret_cast<uintptr_t>(d) & 2) ? 1 : 0;
+        if (odd && lane == 0) {
+            const float v = Vec<S>::load1(s);
+            Vec<T>::store1(d, add ? __fadd_rn(v, Vec<T>::load1(d)) : v);
+        }
+        for (int c0 = odd + 2 * lane; c0 < cols; c0 += 64 * B) {
+            float v[B][2], o[B][2];
 #pragma unroll
-    for (int i = 0; i < per_row; ++i) {
-        const int r = lane / per_row + i * N, c = lane % per_row * N;
-        float f[N];
+            for (int b = 0; b < B; ++b)
 #pragma unroll
-        for (int e = 0; e < N; ++e) f[e] = stage[r * 33 + c + e];
-        put(r, c, f);
+                for (int e = 0; e < 2; ++e) {
+                    const int c = c0 + 64 * b + e;
+                    v[b][e] = c < cols ? Vec<S>::load1(s + c) : 0.f;
+                    o[b][e] = add && c < cols ? Vec<T>::load1(d + c) : 0.f;
+                }
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const int c = c0 + 64 * b;
+                if (c >= cols) continue;
+                const float x = add ? __fadd_rn(v[b][0], o[b][0]) : v[b][0], y = add ? __fadd_rn(v[b][1], o[b][1]) : v[b][1];
+                if (sizeof(T) == 2 && c + 1 < cols) {
+                    *reinterpret_cast<uint32_t*>(d + c) = pack_bf16x2(x, y);
+                } else {
+                    Vec<T>::store1(d + c, x);
+                    if (c + 1 < cols) Vec<T>::store1(d + c + 1, y);
+                }
+            }
+        }
     }
 }
 
 // ---------------------------------------------------------------- the products
-template <int CG>
+// PHASE 0: logits into pairs.  1: logits into g, one plane.  3: g in three planes.  2: dh and dw, one or both.
+template <int CG, int PHASE>
 __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_constant__ CeArgs a) {
-    typedef CeRing<CG> R;
+    typedef CeRing<CG, PHASE> R;
     constexpr int kStages = R::kStages;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], drained;
     __shared__ uint32_t tmem_base;
     __shared__ volatile int abort_flag;
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    __shared__ int hits[8][kHits];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = CG == 1 ? 0 : static_cast<int>(cluster_rank());
     if (threadIdx.x == 0) {
@@ -334,7 +390,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_con
     const uint32_t tmem = tmem_base;
     const int count = *a.count;
     const CeShape s0(a.job[0], count, kTM * CG), s1(a.job[a.jobs - 1], count, kTM * CG);
-    const int total = s0.tiles + (a.jobs > 1 ? s1.tiles : 0);
+    const int total = s0.tiles + (PHASE == 2 && a.jobs > 1 ? s1.tiles : 0);
     const int first = blockIdx.x / CG, stride = gridDim.x / CG;
 
     if (warp == 0) {
@@ -344,7 +400,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_con
             uint32_t wrap = 1;                         // parity of the slot's previous use
             bool ok = true;
             for (int t = first; t < total && ok; t += stride) {
-                const int j = t < s0.tiles ? 0 : 1;
+                const int j = PHASE != 2 || t < s0.tiles ? 0 : 1;
                 const CeTile tile = ce_tile(a.job[j], j ? s1 : s0, j ? t - s0.tiles : t);
                 // everything that the inner loop needs, in registers: one thread feeds the tensor cores of the CTA, and a
                 // division or a load from the argument's memory per slab cost it more than the slab's products take
@@ -403,7 +459,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_con
             const uint32_t ring0 = smem_u32(ring);
             const uint64_t desc = smem_desc(0, kTK * 128);
             for (int t = first; t < total && ok; t += stride, ++n) {
-                const int j = t < s0.tiles ? 0 : 1;
+                const int j = PHASE != 2 || t < s0.tiles ? 0 : 1;
                 const CeTile tile = ce_tile(a.job[j], j ? s1 : s0, j ? t - s0.tiles : t);
                 const uint32_t idesc = mma_idesc(kTM * CG, a.job[j].tn, a.job[j].a_mn, a.job[j].b_mn);
                 const uint32_t step_a = (a.job[j].a_mn ? 2048 : 32) >> 4, step_b = (a.job[j].b_mn ? 2048 : 32) >> 4;
@@ -438,11 +494,12 @@ __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_con
         }
     } else if (warp >= 4) {
         const int quarter = warp & 3, part = (warp - 4) >> 2;     // lanes 32 * quarter.., the part-th half of the columns
-        float* stage = reinterpret_cast<float*>(ring + kStages * R::kStageBytes) + (warp - 4) * kStageFloats;
+        [[maybe_unused]] uint8_t* boxes = ring + kStages * R::kStageBytes + (warp - 4) * R::kBoxes * kBoxBytes;
+        [[maybe_unused]] int turn = 0;
         const uint32_t acc_empty_at[2] = {leader_address(&acc_empty[0]), leader_address(&acc_empty[1])};
         int n = 0;
         for (int t = first; t < total; t += stride, ++n) {
-            const int j = t < s0.tiles ? 0 : 1;
+            const int j = PHASE != 2 || t < s0.tiles ? 0 : 1;
             const CeJob& job = a.job[j];
             const CeShape& sh = j ? s1 : s0;
             const CeTile tile = ce_tile(job, sh, j ? t - s0.tiles : t);
@@ -451,30 +508,11 @@ __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_con
             const bool live = row < sh.m;
             const int c0 = tile.n0 + part * width;
             const int c1 = c0 + width < sh.n ? c0 + width : sh.n;          // this thread's columns that exist
-            // dW: the rows whose target is one of this warp's 32 columns of the vocabulary, found while the products run
-            int n_hits = 0;
-            if (job.epi == kEpiDw && a.left_over) {
-                const int base = a.col0 + row0;
-                for (int i0 = 0; i0 < sh.k; i0 += 128) {
-                    int t[4];
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) t[u] = i0 + 32 * u + lane < sh.k ? a.target[i0 + 32 * u + lane] - base : -1;
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const bool hit = t[u] >= 0 && t[u] < 32;
-                        const uint32_t mask = __ballot_sync(0xffffffffu, hit);
-                        const int at = n_hits + __popc(mask & ((1u << lane) - 1));
-                        if (hit && at < kHits) hits[warp - 4][at] = (i0 + 32 * u + lane) * 32 + t[u];
-                        n_hits += __popc(mask);
-                    }
-                }
-                __syncwarp();
-            }
             if (!wait_or_abort(&acc_full[acc], (n / 2) & 1, &abort_flag, a.status)) break;
             tc_fence_after();
             const uint32_t d = tmem + acc * kTN + part * width + (static_cast<uint32_t>(quarter * 32) << 16);
-            const bool empty_sum = tile.iters == 0;    // nothing was multiplied: the accumulators hold something old
-            if (job.epi == kEpiPairs) {
+            [[maybe_unused]] const bool empty_sum = tile.iters == 0;       // nothing was multiplied: the accumulators hold something old
+            if constexpr (PHASE == 0) {
                 float m = -INFINITY, s = 0.f;
                 const int tgt = live ? a.target[row] - a.col0 : -1;
                 for (int c = c0; c < c0 + width; c += 32) {
@@ -496,130 +534,107 @@ __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_con
                     online_add(v, 1.f, m, s);
                 }
                 if (live) a.pairs[row * a.n_pairs + a.pair0 + c0 / width] = make_float2(m, s);
-            } else if (job.epi == kEpiG) {
-                const int tgt = live ? a.target[row] - a.col0 : -1;
-                const float lse = live ? a.lse[row] : 0.f, gy = live ? a.gy[row] : 0.f;
-                __nv_bfloat16* out = a.g + row0 * a.g_stride;
-                const int64_t plane = a.rows_pad * a.g_stride;
+            } else if constexpr (PHASE == 1 || PHASE == 3) {
                 // columns behind the last one are zeros up to the tile's end: dh and dW read whole slabs of 64
-                const int cz = c0 + width < a.g_stride ? c0 + width : static_cast<int>(a.g_stride);
-                for (int c = c0; c < cz; c += 32) {
+                const int tgt = live ? a.target[row] - a.col0 : -1;
+                const float lse = live ? a.lse[row] : 0.f, gy = live ? __fdiv_rn(a.gy[row], *a.gy_scale) : 0.f;
+#pragma unroll 1
+                for (int c = c0; c < c0 + width; c += 64) {
+#pragma unroll 1
+                    for (int p = 0; p < (PHASE == 3 ? 3 : 1); ++p) {
+                        uint4 w[8];
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const int ch = c + 32 * half;
+                            float v[32];
+                            tmem_load32(d + (ch - c0), v);
+                            const bool here = tgt >= ch && tgt < c1 && tgt < ch + 32;
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) {
+                                float q = ex2f(__fmul_rn(__fsub_rn(v[e], lse), kLog2e));
+                                if (here && tgt == ch + e) q = __fsub_rn(q, 1.f);
+                                v[e] = live && ch + e < c1 ? __fmul_rn(gy, q) : 0.f;
+                            }
+                            if (PHASE == 1 && here) {
+                                float g = 0.f;
+#pragma unroll
+                                for (int e = 0; e < 32; ++e)
+                                    if (tgt == ch + e) g = v[e];
+                                a.left_over[row] = __fsub_rn(g, __bfloat162float(__float2bfloat16_rn(g)));
+                            }
+                            if (PHASE == 3) {          // this plane's 16 bits of each
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) {
+                                    uint32_t hi, mid, lo;
+                                    split3(v[e], hi, mid, lo);
+                                    v[e] = __uint_as_float(p == 0 ? hi : p == 1 ? mid : lo);
+                                }
+                            }
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) w[4 * half + q] = Unit<__nv_bfloat16, 16>::pack(v + 8 * q);
+                        }
+                        ce_send<R::kBoxes>(boxes, turn, w, lane, [&](const uint8_t* box) { tma_store_3d(&a.out[j], box, c, row0, p); });
+                    }
+                }
+            } else if (job.epi == kEpiDh || a.dw_out != kDwScalar) {
+                // rows behind the last one of dh's parts are scratch; those of dW are cut off by the map
+                const bool dh = job.epi == kEpiDh, staged = !dh && a.dw_out == kDwStaged, f32 = dh || a.dw_f32;
+                const float scale = dh ? 1.f : *a.gy_scale;
+                const int step = f32 ? 32 : 64, y = dh || staged ? row0 : a.col0 + row0;
+                // a box that starts behind the last row has nothing to write
+#pragma unroll 1
+                for (int c = c0; c < c1 && row0 < sh.m; c += step) {
+                    uint4 w[8];
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        if (f32 && half) break;
+                        float v[32];
+                        tmem_load32(d + (c - c0) + 32 * half, v);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e] = empty_sum ? 0.f : __fmul_rn(scale, v[e]);
+                        if (f32) {
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) w[q] = Unit<float, 16>::pack(v + 4 * q);
+                        } else {
+                            if (a.dw_add && !staged && live) {
+                                const uint4* o = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.dw) +
+                                                                                static_cast<int64_t>(y + lane) * a.hidden + c + 32 * half);
+#pragma unroll
+                                for (int q = 0; q < 4; ++q)
+                                    if (c + 32 * half + 8 * q < c1) {
+                                        float f[8];
+                                        Unit<__nv_bfloat16, 16>::unpack(o[q], f);
+#pragma unroll
+                                        for (int e = 0; e < 8; ++e) v[8 * q + e] = __fadd_rn(v[8 * q + e], f[e]);
+                                    }
+                            }
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) w[4 * half + q] = Unit<__nv_bfloat16, 16>::pack(v + 8 * q);
+                        }
+                    }
+                    ce_send<R::kBoxes>(boxes, turn, w, lane, [&](const uint8_t* box) {
+                        if (dh ? a.dh_add : (a.dw_add && f32 && !staged)) tma_add_3d(&a.out[j], box, c, y, tile.split);
+                        else tma_store_3d(&a.out[j], box, c, y, tile.split);
+                    });
+                }
+            } else {                                   // a base that TMA cannot write to: element by element
+                const int64_t at = static_cast<int64_t>(a.col0 + row) * a.hidden;
+                const float scale = *a.gy_scale;
+#pragma unroll 1
+                for (int c = c0; c < c1; c += 32) {
                     float v[32];
                     tmem_load32(d + (c - c0), v);
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
-                        const float p = ex2f(__fmul_rn(__fsub_rn(v[e], lse), kLog2e));
-                        v[e] = live && c + e < c1 ? __fmul_rn(gy, tgt == c + e ? __fsub_rn(p, 1.f) : p) : 0.f;
-                    }
-                    if (a.left_over && tgt >= c && tgt < c1 && tgt < c + 32) {
-                        float g = 0.f;
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (tgt == c + e) g = v[e];
-                        a.left_over[row] = __fsub_rn(g, __bfloat162float(__float2bfloat16_rn(g)));
-                    }
-                    ce_store<8>(stage, v, lane, [&](int r, int cc, const float (&f)[8]) {
-                        if (c + cc >= cz) return;
-                        __nv_bfloat16* o = out + r * a.g_stride + c + cc;
-                        if (a.planes == 1) {
-                            *reinterpret_cast<uint4*>(o) = Unit<__nv_bfloat16, 16>::pack(f);
+                        if (!live || c + e >= c1) continue;
+                        const float x = empty_sum ? 0.f : __fmul_rn(scale, v[e]);
+                        if (a.dw_f32) {
+                            float* o = static_cast<float*>(a.dw) + at + c + e;
+                            *o = a.dw_add ? __fadd_rn(x, *o) : x;
                         } else {
-                            uint32_t p0[4], p1[4], p2[4];
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                uint32_t h0, m0, l0, h1, m1, l1;
-                                split3(f[2 * q], h0, m0, l0);
-                                split3(f[2 * q + 1], h1, m1, l1);
-                                p0[q] = (h0 >> 16) | h1;
-                                p1[q] = (m0 >> 16) | m1;
-                                p2[q] = (l0 >> 16) | l1;
-                            }
-                            *reinterpret_cast<uint4*>(o) = make_uint4(p0[0], p0[1], p0[2], p0[3]);
-                            *reinterpret_cast<uint4*>(o + plane) = make_uint4(p1[0], p1[1], p1[2], p1[3]);
-                            *reinterpret_cast<uint4*>(o + 2 * plane) = make_uint4(p2[0], p2[1], p2[2], p2[3]);
+                            __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.dw) + at + c + e;
+                            *o = __float2bfloat16_rn(a.dw_add ? __fadd_rn(x, __bfloat162float(*o)) : x);
                         }
-                    });
-                }
-            } else if (job.epi == kEpiDh) {
-                float* out = a.dh + (static_cast<int64_t>(tile.split) * a.rows_pad + row0) * a.dh_stride;
-                for (int c = c0; c < c1; c += 32) {
-                    float v[32];
-                    tmem_load32(d + (c - c0), v);
-                    ce_store<4>(stage, v, lane, [&](int r, int cc, const float (&f)[4]) {
-                        if (row0 + r >= sh.m || c + cc >= c1) return;         // the stride is the width rounded up to 4
-                        float4* o = reinterpret_cast<float4*>(out + r * a.dh_stride + c + cc);
-                        float4 w = empty_sum ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(f[0], f[1], f[2], f[3]);
-                        if (a.dh_add) {
-                            const float4 old = *o;
-                            w = make_float4(__fadd_rn(old.x, w.x), __fadd_rn(old.y, w.y), __fadd_rn(old.z, w.z), __fadd_rn(old.w, w.w));
-                        }
-                        *o = w;
-                    });
-                }
-            } else {
-                const int64_t at = static_cast<int64_t>(a.col0 + row0) * a.hidden;
-                const bool vec = a.hidden % 8 == 0 && (reinterpret_cast<uintptr_t>(a.dw) & 15) == 0;
-                for (int c = c0; c < c1; c += 32) {
-                    float v[32];
-                    tmem_load32(d + (c - c0), v);
-                    if (empty_sum) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) v[e] = 0.f;
-                    }
-                    auto add_left_over = [&](int i) {
-                        const float left = a.left_over[i];
-                        const uint4* h = reinterpret_cast<const uint4*>(a.h + i * a.h_stride + c);
-#pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            if (c + 8 * q < c1) {
-                                float f[8];
-                                Unit<__nv_bfloat16, 16>::unpack(h[q], f);
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) v[8 * q + e] = __fmaf_rn(left, f[e], v[8 * q + e]);
-                            }
-                    };
-                    if (n_hits <= kHits) {
-                        for (int k = 0; k < n_hits; ++k) {
-                            const int x = hits[warp - 4][k];
-                            if ((x & 31) == lane) add_left_over(x >> 5);
-                        }
-                    } else {                           // more than the list holds: all targets once more, in the same order
-                        for (int i = 0; i < sh.k; ++i)
-                            if (a.target[i] - a.col0 == row) add_left_over(i);
-                    }
-                    if (!vec) {
-                        ce_store<1>(stage, v, lane, [&](int r, int cc, const float (&f)[1]) {
-                            if (row0 + r >= sh.m || c + cc >= c1) return;
-                            const int64_t o = at + static_cast<int64_t>(r) * a.hidden + c + cc;
-                            if (a.dw_f32) {
-                                float* w = static_cast<float*>(a.dw) + o;
-                                *w = a.dw_add ? __fadd_rn(f[0], *w) : f[0];
-                            } else {
-                                __nv_bfloat16* w = static_cast<__nv_bfloat16*>(a.dw) + o;
-                                *w = __float2bfloat16_rn(a.dw_add ? __fadd_rn(f[0], __bfloat162float(*w)) : f[0]);
-                            }
-                        });
-                    } else if (a.dw_f32) {
-                        ce_store<4>(stage, v, lane, [&](int r, int cc, const float (&f)[4]) {
-                            if (row0 + r >= sh.m || c + cc >= c1) return;
-                            float4* o = reinterpret_cast<float4*>(static_cast<float*>(a.dw) + at + static_cast<int64_t>(r) * a.hidden + c + cc);
-                            float4 w = make_float4(f[0], f[1], f[2], f[3]);
-                            if (a.dw_add) {
-                                const float4 old = *o;
-                                w = make_float4(__fadd_rn(old.x, w.x), __fadd_rn(old.y, w.y), __fadd_rn(old.z, w.z), __fadd_rn(old.w, w.w));
-                            }
-                            __stcs(o, w);
-                        });
-                    } else {
-                        ce_store<8>(stage, v, lane, [&](int r, int cc, const float (&f)[8]) {
-                            if (row0 + r >= sh.m || c + cc >= c1) return;
-                            uint4* o = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.dw) + at + static_cast<int64_t>(r) * a.hidden + c + cc);
-                            float w[8];
-                            if (a.dw_add) Unit<__nv_bfloat16, 16>::unpack(*o, w);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) w[e] = a.dw_add ? __fadd_rn(f[e], w[e]) : f[e];
-                            store_vec_streaming(o, Unit<__nv_bfloat16, 16>::pack(w));
-                        });
                     }
                 }
             }
@@ -630,6 +645,7 @@ __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_con
                 else mbar_arrive_cluster(acc_empty_at[acc]);
             }
         }
+        tma_store_wait();                              // this thread's boxes have been written
     }
     __syncwarp();
     tc_fence_before();
@@ -693,7 +709,9 @@ __global__ void __launch_bounds__(256) ce_join_kernel(const float2* pairs, int n
 // the row took no part.  A thread takes four neighbouring columns.
 template <typename T>
 __global__ void __launch_bounds__(256) ce_dh_kernel(const float* parts, int splits, int64_t rows_pad, int64_t stride, const int* pos_of,
-                                                    const int* target_of, const float* left_over, const T* w, T* dh, int64_t rows, int hidden) {
+                                                    const int* target_of, const float* left_over, const float* gy_scale, const T* w, T* dh,
+                                                    int64_t rows, int hidden) {
+    const float scale = *gy_scale;
     const int quads = (hidden + 3) / 4;
     const bool vec = sizeof(T) == 4 ? hidden % 4 == 0 && (reinterpret_cast<uintptr_t>(dh) & 15) == 0
                                     : hidden % 4 == 0 && (reinterpret_cast<uintptr_t>(dh) & 7) == 0;
@@ -718,6 +736,8 @@ __global__ void __launch_bounds__(256) ce_dh_kernel(const float* parts, int spli
                         if (4 * q + e < hidden) s[e] = __fmaf_rn(left, Vec<T>::load1(wr + 4 * q + e), s[e]);
                 }
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] = __fmul_rn(scale, s[e]);
             T* o = dh + r * hidden + 4 * q;
             if (vec && sizeof(T) == 4) {
                 *reinterpret_cast<float4*>(o) = make_float4(s[0], s[1], s[2], s[3]);

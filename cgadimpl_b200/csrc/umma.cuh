@@ -99,9 +99,8 @@ __device__ __forceinline__ void tmem_free(uint32_t base, uint32_t columns) {
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// 32 columns of this thread's lane (the warp's quarter of the 128 lanes), fp32.
-__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
-    uint32_t r[32];
+// 32 columns of this thread's lane (the warp's quarter of the 128 lanes), fp32.  The values may be read after tmem_wait().
+__device__ __forceinline__ void tmem_load32_async(uint32_t addr, uint32_t (&r)[32]) {
     __syncwarp();                                      // .aligned: the whole warp, together
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -112,10 +111,36 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
           "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
           "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
+    uint32_t r[32];
+    tmem_load32_async(addr, r);
+    tmem_wait();
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
+
+// ---------------------------------------------------------------- tiled TMA store
+// A box of 128-byte rows from shared memory (128-byte swizzle) to coordinates (x, y, z); what lies beyond the tensor is not written.
+// One thread issues it after every writer's fence_async() and a barrier between them.
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(smem_u32(src)), "r"(x),
+                 "r"(y), "r"(z)
+                 : "memory");
+}
+// The same, added to fp32 values in place.
+__device__ __forceinline__ void tma_add_3d(const CUtensorMap* map, const void* src, int x, int y, int z) {
+    asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
+                 "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// All but the last N groups of this thread have been read from shared memory.
+template <int N>
+__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // ---------------------------------------------------------------- descriptors
 // Shared-memory matrix descriptor, 128-byte swizzle (layout 2), descriptor version 1.
