@@ -3,6 +3,8 @@
 #define AGB_NO_STATUS_WORD
 #include <nvtx3/nvToolsExt.h>
 
+#include <type_traits>
+
 #include "agb/agb.h"
 #include "agb_internal.h"
 #include "distill_topk.cuh"
@@ -36,6 +38,33 @@ struct NvtxRange {
 
 inline uintptr_t addr(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Launches with programmatic stream serialization (the kernels call pdl_wait() before they touch what the one before wrote) and, where
+// `cluster` is above 1, in clusters.
+template <typename... KArgs, typename... Args>
+int launch(const char* what, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster, Args... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (agb_int::pdl_enabled()) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = cluster;
+        attr[n].val.clusterDim.y = 1;
+        attr[n++].val.clusterDim.z = 1;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    AGB_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...));
+    return after_launch(what);
+}
 
 // ------------------------------------------------------------------ LayerNorm with weight and bias
 int check_lna(int64_t rows, int64_t hidden, int dtype) {
@@ -139,19 +168,7 @@ int launch_kd(agb::KdArgs a, int64_t rows, cudaStream_t st) {
     int C = 1;
     while (C < 8 && rows * C < 2 * d.sms && a.vocab / (2 * C) >= agb::kKdThreads * (16 / static_cast<int>(sizeof(T)))) C *= 2;
     a.slice = ceil_div(ceil_div(a.vocab, C), 64) * 64;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(rows * C));
-    cfg.blockDim = dim3(agb::kKdThreads);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = C;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    AGB_CUDA(cudaLaunchKernelEx(&cfg, agb::kd_kernel<T, MODE>, a));
-    return after_launch("distill_topk");
+    return launch("distill_topk", agb::kd_kernel<T, MODE>, dim3(static_cast<unsigned>(rows * C)), dim3(agb::kKdThreads), 0, st, C, a);
 }
 
 template <int MODE>
@@ -355,35 +372,33 @@ int ce_rows(const CeCall& c, const float* lse, const float* gy, float* loss, flo
     a.lse_out = lse_out;
     // a warp per row while the blocks, which all count the targets before their own, stay about a thousand
     a.per_block = c.rows <= 8192 ? 8 : c.rows <= 16384 ? 16 : agb::kRowsBlock;
-    const unsigned grid = static_cast<unsigned>(ceil_div(c.rows, a.per_block));
-    if (c.dtype == AGB_F32) agb::ce_rows_kernel<float><<<grid, 256, 0, c.st>>>(a);
-    else agb::ce_rows_kernel<bf16><<<grid, 256, 0, c.st>>>(a);
-    return after_launch("linear_ce_rows");
+    const dim3 grid(static_cast<unsigned>(ceil_div(c.rows, a.per_block)) + agb::kRowsEnd);
+    return launch("linear_ce_rows", c.dtype == AGB_F32 ? agb::ce_rows_kernel<float> : agb::ce_rows_kernel<bf16>, grid, dim3(256), 0, c.st, 1, a);
 }
 int ce_pack(const CeCall& c, int64_t col0, int64_t n) {
     if (c.p.direct_w) return AGB_OK;
     int64_t grid = ceil_div(n, 8);
     if (grid > 16LL * c.d.sms) grid = 16LL * c.d.sms;
+    const dim3 g(static_cast<unsigned>(grid)), block(256);
+    const int cols = static_cast<int>(c.hidden);
     if (c.dtype == AGB_F32)
-        agb::ce_pack_kernel<float><<<static_cast<unsigned>(grid), 256, 0, c.st>>>(static_cast<const float*>(c.w) + col0 * c.hidden, n, (int)c.hidden,
-                                                                                 c.at<bf16>(c.p.w), c.p.piece, c.p.k_stride);
-    else
-        agb::ce_pack_kernel<bf16><<<static_cast<unsigned>(grid), 256, 0, c.st>>>(static_cast<const bf16*>(c.w) + col0 * c.hidden, n, (int)c.hidden,
-                                                                                c.at<bf16>(c.p.w), c.p.piece, c.p.k_stride);
-    return after_launch("linear_ce_pack");
+        return launch("linear_ce_pack", agb::ce_pack_kernel<float>, g, block, 0, c.st, 1, static_cast<const float*>(c.w) + col0 * c.hidden, n, cols,
+                      c.at<bf16>(c.p.w), c.p.piece, c.p.k_stride);
+    return launch("linear_ce_pack", agb::ce_pack_kernel<bf16>, g, block, 0, c.st, 1, static_cast<const bf16*>(c.w) + col0 * c.hidden, n, cols,
+                  c.at<bf16>(c.p.w), c.p.piece, c.p.k_stride);
 }
 int ce_unpack(const CeCall& c, void* dw, int64_t col0, int64_t n, bool f32, int add) {
     int64_t grid = ceil_div(n, 8);
     if (grid > 16LL * c.d.sms) grid = 16LL * c.d.sms;
-    const unsigned g = static_cast<unsigned>(grid);
+    const dim3 g(static_cast<unsigned>(grid)), block(256);
     const int cols = static_cast<int>(c.hidden);
+    const char* what = "linear_ce_unpack";
     if (c.dtype == AGB_F32)
-        agb::ce_unpack_kernel<float, float><<<g, 256, 0, c.st>>>(c.at<float>(c.p.dw), n, cols, c.p.k_stride, static_cast<float*>(dw) + col0 * c.hidden, add);
-    else if (f32)
-        agb::ce_unpack_kernel<float, bf16><<<g, 256, 0, c.st>>>(c.at<float>(c.p.dw), n, cols, c.p.k_stride, static_cast<bf16*>(dw) + col0 * c.hidden, add);
-    else
-        agb::ce_unpack_kernel<bf16, bf16><<<g, 256, 0, c.st>>>(c.at<bf16>(c.p.dw), n, cols, c.p.k_stride, static_cast<bf16*>(dw) + col0 * c.hidden, add);
-    return after_launch("linear_ce_unpack");
+        return launch(what, agb::ce_unpack_kernel<float, float>, g, block, 0, c.st, 1, c.at<float>(c.p.dw), n, cols, c.p.k_stride,
+                      static_cast<float*>(dw) + col0 * c.hidden, add);
+    bf16* to = static_cast<bf16*>(dw) + col0 * c.hidden;
+    if (f32) return launch(what, agb::ce_unpack_kernel<float, bf16>, g, block, 0, c.st, 1, c.at<float>(c.p.dw), n, cols, c.p.k_stride, to, add);
+    return launch(what, agb::ce_unpack_kernel<bf16, bf16>, g, block, 0, c.st, 1, c.at<bf16>(c.p.dw), n, cols, c.p.k_stride, to, add);
 }
 // W, or its piece where it was laid out: rows of the map, and the map's row of the piece's first column.
 int map_w(const CeCall& c, CUtensorMap* m, int64_t n, int box_rows) {
@@ -432,20 +447,8 @@ int launch_gemm_cg(const CeCall& c, const agb::CeArgs& a) {
     if (tiles >= (1LL << 31)) return fail(AGB_ERR_UNSUPPORTED, "too many tiles");
     AGB_CUDA(cudaFuncSetAttribute(agb::ce_gemm_kernel<CG, PHASE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (agb::CeRing<CG, PHASE>::kSmem)));
     const int64_t most = c.d.sms / CG;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>((tiles < most ? tiles : most) * CG));
-    cfg.blockDim = dim3(agb::kCeThreads);
-    cfg.dynamicSmemBytes = (agb::CeRing<CG, PHASE>::kSmem);
-    cfg.stream = c.st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CG;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    AGB_CUDA(cudaLaunchKernelEx(&cfg, agb::ce_gemm_kernel<CG, PHASE>, a));
-    return after_launch("linear_ce_gemm");
+    return launch("linear_ce_gemm", agb::ce_gemm_kernel<CG, PHASE>, dim3(static_cast<unsigned>((tiles < most ? tiles : most) * CG)),
+                  dim3(agb::kCeThreads), agb::CeRing<CG, PHASE>::kSmem, c.st, CG, a);
 }
 template <int PHASE>
 int launch_gemm(const CeCall& c, const agb::CeArgs& a) {
@@ -505,16 +508,17 @@ int agb_linear_ce_fwd(const void* h, const void* w, const void* target, int targ
     }
     const int64_t last = vocab - (c.p.pieces - 1) * c.p.piece;
     const int pairs = static_cast<int>((c.p.pieces - 1) * c.p.pairs_per_piece + ceil_div(last, c.p.tn) * 2);
-    const unsigned grid = static_cast<unsigned>(ceil_div(rows, 8));
+    const bool few = rows <= 8LL * c.d.sms;
+    const dim3 grid(static_cast<unsigned>(few ? rows : ceil_div(rows, 8)));
+    auto join = [&](auto kernel, auto* typed) {
+        typedef decltype(typed) P;
+        return launch("linear_ce_join", kernel, grid, dim3(256), 0, c.st, 1, c.at<float2>(c.p.pair_at), pairs, c.p.pairs, c.at<int>(c.p.count),
+                      c.at<float>(c.p.z_target), c.at<int>(c.p.target_of), c.at<int>(c.p.row_of), static_cast<P>(h), static_cast<P>(w),
+                      static_cast<int>(hidden), loss, lse);
+    };
     if (dtype == AGB_F32)
-        agb::ce_join_kernel<float><<<grid, 256, 0, c.st>>>(c.at<float2>(c.p.pair_at), pairs, c.p.pairs, c.at<int>(c.p.count), c.at<float>(c.p.z_target),
-                                                           c.at<int>(c.p.target_of), c.at<int>(c.p.row_of), static_cast<const float*>(h),
-                                                           static_cast<const float*>(w), (int)hidden, loss, lse);
-    else
-        agb::ce_join_kernel<bf16><<<grid, 256, 0, c.st>>>(c.at<float2>(c.p.pair_at), pairs, c.p.pairs, c.at<int>(c.p.count), c.at<float>(c.p.z_target),
-                                                          c.at<int>(c.p.target_of), c.at<int>(c.p.row_of), static_cast<const bf16*>(h),
-                                                          static_cast<const bf16*>(w), (int)hidden, loss, lse);
-    return after_launch("linear_ce_join");
+        return join(few ? agb::ce_join_kernel<float, 8> : agb::ce_join_kernel<float, 1>, static_cast<const float*>(nullptr));
+    return join(few ? agb::ce_join_kernel<bf16, 8> : agb::ce_join_kernel<bf16, 1>, static_cast<const bf16*>(nullptr));
 }
 
 int agb_linear_ce_bwd(const void* h, const void* w, const void* target, int target_type, const float* lse, const float* gy, void* dh,
@@ -614,15 +618,13 @@ int agb_linear_ce_bwd(const void* h, const void* w, const void* target, int targ
     if (dh) {
         const dim3 grid(static_cast<unsigned>(ceil_div(ceil_div(hidden, 4), 256)), static_cast<unsigned>(rows < 32768 ? rows : 32768));
         const float* left = c.p.planes == 1 ? c.at<float>(c.p.left_over) : nullptr;
-        if (dtype == AGB_F32)
-            agb::ce_dh_kernel<float><<<grid, 256, 0, c.st>>>(c.at<float>(c.p.dh), c.p.splits, c.p.rows_pad, c.p.dh_stride, c.at<int>(c.p.pos_of),
-                                                             c.at<int>(c.p.target_of), left, c.at<float>(c.p.gy_scale), static_cast<const float*>(w), static_cast<float*>(dh),
-                                                             rows, (int)hidden);
-        else
-            agb::ce_dh_kernel<bf16><<<grid, 256, 0, c.st>>>(c.at<float>(c.p.dh), c.p.splits, c.p.rows_pad, c.p.dh_stride, c.at<int>(c.p.pos_of),
-                                                            c.at<int>(c.p.target_of), left, c.at<float>(c.p.gy_scale), static_cast<const bf16*>(w), static_cast<bf16*>(dh),
-                                                            rows, (int)hidden);
-        return after_launch("linear_ce_dh");
+        auto add_up = [&](auto kernel, auto* to) {
+            typedef std::remove_pointer_t<decltype(to)> T;
+            return launch("linear_ce_dh", kernel, grid, dim3(256), 0, c.st, 1, c.at<float>(c.p.dh), c.p.splits, c.p.rows_pad, c.p.dh_stride,
+                          c.at<int>(c.p.pos_of), c.at<int>(c.p.target_of), left, c.at<float>(c.p.gy_scale), static_cast<const T*>(w), to, rows,
+                          static_cast<int>(hidden));
+        };
+        return dtype == AGB_F32 ? add_up(agb::ce_dh_kernel<float>, static_cast<float*>(dh)) : add_up(agb::ce_dh_kernel<bf16>, static_cast<bf16*>(dh));
     }
     return AGB_OK;
 }

@@ -85,6 +85,8 @@ __global__ void __launch_bounds__(kKdThreads) kd_kernel(const KdArgs a) {
     const int64_t hi = lo + a.slice < a.vocab ? lo + a.slice : a.vocab;
     const T* add = (MODE > 0 && a.dz_add) ? static_cast<const T*>(a.dz_add) + r * a.vocab : nullptr;
 
+    pdl_wait();
+    pdl_trigger();
     // ---- the teacher's row: p_k in shared memory, the same bits in every CTA
     float tmax = -INFINITY;
     for (int k = tid; k < a.k; k += kKdThreads) {

@@ -152,7 +152,8 @@ __device__ __forceinline__ void split3(float x, uint32_t& hi, uint32_t& mid, uin
 // Rows of x [rows][cols] whose target names a column, in order and without gaps, into dst [planes][rows_pad][stride] bf16;
 // zeros behind the last column up to `stride` and, for the backward, behind the last row up to a multiple of kTK.  Also the
 // per-row arrays.
-// A block takes `per_block` (at most 32) rows; it counts the targets before its own to know where they go.
+// A block takes `per_block` (at most 32) rows; it counts the targets before its own to know where they go.  kRowsEnd blocks behind them
+// count all targets and do what needs that number.
 struct CeRowsArgs {
     const void* x;
     const void* target;
@@ -170,6 +171,7 @@ struct CeRowsArgs {
     float *loss, *lse_out;             // forward: rows that take no part get 0
 };
 constexpr int kRowsBlock = 32;         // most rows of a block
+constexpr int kRowsEnd = 8;
 
 __device__ __forceinline__ int ce_target(const CeRowsArgs& a, int64_t r) {
     const int64_t t = a.target64 ? static_cast<const int64_t*>(a.target)[r] : static_cast<const int32_t*>(a.target)[r];
@@ -228,46 +230,32 @@ template <typename T>
 __global__ void __launch_bounds__(256) ce_rows_kernel(const CeRowsArgs a) {
     __shared__ int warp_count[8];
     __shared__ int where[kRowsBlock];
-    __shared__ int last;
     __shared__ float scale_of[8];
-    const int64_t r0 = static_cast<int64_t>(blockIdx.x) * a.per_block;
+    pdl_wait();
+    pdl_trigger();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t plane = a.rows_pad * a.stride;
+    const int end = static_cast<int>(blockIdx.x) - (static_cast<int>(gridDim.x) - kRowsEnd);   // >= 0: one of the last blocks
+    const int64_t r0 = end >= 0 ? a.rows : static_cast<int64_t>(blockIdx.x) * a.per_block;
     int n = 0;
 #pragma unroll 4
     for (int64_t r = threadIdx.x; r < r0; r += 256) n += ce_target(a, r) >= 0;
     n = __reduce_add_sync(0xffffffffu, n);
-    if ((threadIdx.x & 31) == 0) warp_count[threadIdx.x >> 5] = n;
+    if (lane == 0) warp_count[warp] = n;
     __syncthreads();
     int base = 0;
     for (int w = 0; w < 8; ++w) base += warp_count[w];
-    if (threadIdx.x < 32) {
-        const int64_t r = r0 + threadIdx.x;
-        const int t = threadIdx.x < a.per_block && r < a.rows ? ce_target(a, r) : -1;
-        const uint32_t mask = __ballot_sync(0xffffffffu, t >= 0);
-        const int at = base + __popc(mask & ((1u << threadIdx.x) - 1));
-        where[threadIdx.x] = t >= 0 ? at : -1;
-        if (t >= 0) {
-            a.row_of[at] = static_cast<int>(r);
-            a.target_of[at] = t;
-            if (a.lse) {
-                a.lse_of[at] = a.lse[r];
-                a.gy_of[at] = a.gy[r];
-            }
-        } else if (threadIdx.x < a.per_block && r < a.rows && a.loss) {
-            a.loss[r] = 0.f;
-            a.lse_out[r] = 0.f;
+    if (end >= 0) {
+        if (a.lse) {                                   // rows of dW's sum behind the last one, up to a whole slab, are zeros
+            const int stop = (base + kTK - 1) / kTK * kTK;
+            for (int p = 0; p < a.planes; ++p)
+                for (int i = base + end; i < stop; i += kRowsEnd) {
+                    uint4* d = reinterpret_cast<uint4*>(a.dst + p * plane + i * a.stride);
+                    for (int64_t c = threadIdx.x; c < a.stride / 8; c += 256) d[c] = make_uint4(0, 0, 0, 0);
+                }
         }
-        if (threadIdx.x < a.per_block && r < a.rows) a.pos_of[r] = t >= 0 ? at : -1;
-        if (threadIdx.x == 0) last = base + __popc(mask);
-    }
-    __syncthreads();
-    const int64_t plane = a.rows_pad * a.stride;
-    const bool vec = sizeof(T) == 2 && a.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int i = warp; i < a.per_block; i += 8)
-        if (where[i] >= 0)
-            ce_copy_row(static_cast<const T*>(a.x) + (r0 + i) * a.cols, a.dst + where[i] * a.stride, a.cols, a.stride, plane, vec, lane);
-    if (blockIdx.x + 1 == gridDim.x) {                 // the last block knows the number of rows
-        if (threadIdx.x == 0) *a.count = last;
+        if (end > 0) return;
+        if (threadIdx.x == 0) *a.count = base;
         if (a.lse) {                                   // the largest |gy| of the rows that take part, 1 where that is no scale
             float top = 0.f;
 #pragma unroll 4
@@ -281,18 +269,40 @@ __global__ void __launch_bounds__(256) ce_rows_kernel(const CeRowsArgs a) {
                 *a.gy_scale = top > 0x1p-100f && top < 0x1p100f ? top : 1.f;
             }
         }
-        // rows of dW's sum behind the last one, up to a whole slab
-        const int64_t stop = (static_cast<int64_t>(last) + kTK - 1) / kTK * kTK;
-        for (int p = 0; a.lse && p < a.planes; ++p) {
-            uint4* d = reinterpret_cast<uint4*>(a.dst + p * plane + last * a.stride);
-            for (int64_t i = threadIdx.x; i < (stop - last) * a.stride / 8; i += 256) d[i] = make_uint4(0, 0, 0, 0);
-        }
+        return;
     }
+    if (threadIdx.x < 32) {
+        const int64_t r = r0 + threadIdx.x;
+        const bool mine = threadIdx.x < a.per_block && r < a.rows;
+        const int t = mine ? ce_target(a, r) : -1;
+        const uint32_t mask = __ballot_sync(0xffffffffu, t >= 0);
+        const int at = base + __popc(mask & ((1u << threadIdx.x) - 1));
+        where[threadIdx.x] = t >= 0 ? at : -1;
+        if (t >= 0) {
+            a.row_of[at] = static_cast<int>(r);
+            a.target_of[at] = t;
+            if (a.lse) {
+                a.lse_of[at] = a.lse[r];
+                a.gy_of[at] = a.gy[r];
+            }
+        } else if (mine && a.loss) {
+            a.loss[r] = 0.f;
+            a.lse_out[r] = 0.f;
+        }
+        if (mine) a.pos_of[r] = t >= 0 ? at : -1;
+    }
+    __syncthreads();
+    const bool vec = sizeof(T) == 2 && a.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
+    for (int i = warp; i < a.per_block; i += 8)
+        if (where[i] >= 0)
+            ce_copy_row(static_cast<const T*>(a.x) + (r0 + i) * a.cols, a.dst + where[i] * a.stride, a.cols, a.stride, plane, vec, lane);
 }
 
 // Rows [row0, row0 + rows) of w into dst [planes][rows_pad][stride]: what W needs where TMA cannot read it as it is.
 template <typename T>
 __global__ void __launch_bounds__(256) ce_pack_kernel(const T* w, int64_t rows, int cols, __nv_bfloat16* dst, int64_t rows_pad, int64_t stride) {
+    pdl_wait();
+    pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + warp; r < rows; r += static_cast<int64_t>(gridDim.x) * 8)
         ce_copy_row(w + r * cols, dst + r * stride, cols, stride, rows_pad * stride, false, lane);
@@ -321,6 +331,8 @@ __device__ __forceinline__ void ce_send(uint8_t* boxes, int& turn, const uint4 (
 template <typename S, typename T>
 __global__ void __launch_bounds__(256) ce_unpack_kernel(const S* src, int64_t rows, int cols, int64_t stride, T* dw, int add) {
     constexpr int B = 8;
+    pdl_wait();
+    pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + warp; r < rows; r += static_cast<int64_t>(gridDim.x) * 8) {
         const S* s = src + r * stride;
@@ -388,6 +400,8 @@ __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_con
     if (CG == 2) cluster_barrier();                    // the leader's barriers are ready before the other CTA's copies arrive
     tc_fence_after();
     const uint32_t tmem = tmem_base;
+    pdl_wait();                                        // barriers and tensor memory were set up under the kernel before
+    pdl_trigger();
     const int count = *a.count;
     const CeShape s0(a.job[0], count, kTM * CG), s1(a.job[a.jobs - 1], count, kTM * CG);
     const int total = s0.tiles + (PHASE == 2 && a.jobs > 1 ? s1.tiles : 0);
@@ -656,41 +670,51 @@ __global__ void __launch_bounds__(kCeThreads, 1) ce_gemm_kernel(const __grid_con
 }
 
 // ---------------------------------------------------------------- joining
-// lse and loss of the rows that take part, a warp per row.  The loss is a difference of two numbers of the size of the logits, and the
-// tensor cores cut (not round) every partial sum: z_target there was off by 1.5e-5 at 4096 terms of one sign.  So z_target is computed
-// once more, in fp32, and takes its own place in the sum of exponentials as well: the two agree, and the loss of a target with p near one
-// is not a difference of two errors.
-template <typename T>
+// lse and loss of the rows that take part, W warps per row (one where rows fill the GPU, eight where they are few).  The loss is a
+// difference of two numbers of the size of the logits, and the tensor cores cut (not round) every partial sum: z_target there was off by
+// 1.5e-5 at 4096 terms of one sign.  So z_target is computed once more, in fp32, and takes its own place in the sum of exponentials as
+// well: the two agree, and the loss of a target with p near one is not a difference of two errors.
+template <typename T, int W>
 __global__ void __launch_bounds__(256) ce_join_kernel(const float2* pairs, int n, int64_t n_pairs, const int* count, const float* z_target,
                                                       const int* target_of, const int* row_of, const T* h, const T* w, int hidden, float* loss,
                                                       float* lse) {
-    const int i = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (i >= *count) return;
-    const int r = row_of[i];
-    const T* hr = h + static_cast<int64_t>(r) * hidden;
-    const T* wr = w + static_cast<int64_t>(target_of[i]) * hidden;
+    __shared__ float part[8][3];
+    // what the dot product reads was written before the products started: it runs under their end
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int i = blockIdx.x * (8 / W) + warp / W, me = threadIdx.x % (32 * W);
+    const bool live = i < *count;                      // the same for all threads of the block where W > 1
     typedef Unit<T, 16> U;
     float z = 0.f;
-    if (hidden % U::N == 0 && ((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(w)) & 15) == 0) {
-        const uint4* hv = reinterpret_cast<const uint4*>(hr);
-        const uint4* wv = reinterpret_cast<const uint4*>(wr);
+    int r = 0;
+    if (live) {
+        r = row_of[i];
+        const T* hr = h + static_cast<int64_t>(r) * hidden;
+        const T* wr = w + static_cast<int64_t>(target_of[i]) * hidden;
+        if (hidden % U::N == 0 && ((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(w)) & 15) == 0) {
+            const uint4* hv = reinterpret_cast<const uint4*>(hr);
+            const uint4* wv = reinterpret_cast<const uint4*>(wr);
 #pragma unroll 4
-        for (int c = lane; c < hidden / U::N; c += 32) {
-            float f[U::N], g[U::N];
-            U::unpack(hv[c], f);
-            U::unpack(wv[c], g);
+            for (int c = me; c < hidden / U::N; c += 32 * W) {
+                float f[U::N], g[U::N];
+                U::unpack(hv[c], f);
+                U::unpack(wv[c], g);
 #pragma unroll
-            for (int e = 0; e < U::N; ++e) z = __fmaf_rn(f[e], g[e], z);
-        }
-    } else {
+                for (int e = 0; e < U::N; ++e) z = __fmaf_rn(f[e], g[e], z);
+            }
+        } else {
 #pragma unroll 8
-        for (int c = lane; c < hidden; c += 32) z = __fmaf_rn(Vec<T>::load1(hr + c), Vec<T>::load1(wr + c), z);
+            for (int c = me; c < hidden; c += 32 * W) z = __fmaf_rn(Vec<T>::load1(hr + c), Vec<T>::load1(wr + c), z);
+        }
     }
+    pdl_wait();
+    pdl_trigger();
     float m = -INFINITY, s = 0.f;
+    if (live) {
 #pragma unroll 4
-    for (int p = lane; p < n; p += 32) {
-        const float2 q = pairs[i * n_pairs + p];
-        join_pair(m, s, q.x, q.y);
+        for (int p = me; p < n; p += 32 * W) {
+            const float2 q = pairs[i * n_pairs + p];
+            join_pair(m, s, q.x, q.y);
+        }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -698,7 +722,20 @@ __global__ void __launch_bounds__(256) ce_join_kernel(const float2* pairs, int n
         const float mb = __shfl_xor_sync(0xffffffffu, m, o), sb = __shfl_xor_sync(0xffffffffu, s, o);
         join_pair(m, s, mb, sb);
     }
-    if (lane) return;
+    if (W > 1) {
+        if (lane == 0) {
+            part[warp][0] = z;
+            part[warp][1] = m;
+            part[warp][2] = s;
+        }
+        __syncthreads();
+        if (warp) return;
+        for (int q = 1; q < W; ++q) {
+            z = __fadd_rn(z, part[q][0]);
+            join_pair(m, s, part[q][1], part[q][2]);
+        }
+    }
+    if (lane || !live) return;
     s = __fadd_rn(s, __fsub_rn(exp2f(__fmul_rn(__fsub_rn(z, m), kLog2e)), exp2f(__fmul_rn(__fsub_rn(z_target[i], m), kLog2e))));
     const float l = __fadd_rn(m, logf(s));
     lse[r] = l;
@@ -711,6 +748,8 @@ template <typename T>
 __global__ void __launch_bounds__(256) ce_dh_kernel(const float* parts, int splits, int64_t rows_pad, int64_t stride, const int* pos_of,
                                                     const int* target_of, const float* left_over, const float* gy_scale, const T* w, T* dh,
                                                     int64_t rows, int hidden) {
+    pdl_wait();
+    pdl_trigger();
     const float scale = *gy_scale;
     const int quads = (hidden + 3) / 4;
     const bool vec = sizeof(T) == 4 ? hidden % 4 == 0 && (reinterpret_cast<uintptr_t>(dh) & 15) == 0
