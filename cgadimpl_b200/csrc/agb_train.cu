@@ -109,40 +109,99 @@ int lna_fwd(agb::LnaFwdArgs a, int sms, cudaStream_t st) {
     return after_launch("layernorm_affine_fwd");
 }
 
-template <typename T, int UB>
-int lna_dx(agb::LnaBwdArgs a, int sms, cudaStream_t st) {
-    constexpr int N = agb::Unit<T, UB>::N, UPT = 16 / N;
-    a.G = threads_per_row(a.hidden / N, UPT, 512);
-    if (a.G) {
-        const int block = a.G <= 32 ? 128 : a.G;
-        agb::lna_dx_kernel<T, UB, UPT><<<static_cast<unsigned>(grid_for(a.rows, a.G, block, sms, 2048 / block)), block, 0, st>>>(a);
-    } else {
-        agb::lna_dx_wide<T, UB><<<static_cast<unsigned>(grid_for(a.rows, 1024, 1024, sms, 2)), 1024, 0, st>>>(a);
-    }
-    return after_launch("layernorm_affine_bwd");
+constexpr int kLnaRuns = 64;        // wide rows: runs of rows of the column sums, each a partial row
+constexpr int kLnaCtas = 4;         // most CTAs per SM of the ring kernel
+// Partial rows that a workspace has room for: four CTAs on each of 160 SMs, two where a row is long.
+int64_t lna_partials(int64_t rows, int64_t hidden) {
+    const int64_t most = hidden <= 2048 ? 640 : 320;
+    return rows < 1 ? 1 : rows < most ? rows : most;
 }
 
-constexpr int kLnaRuns = 64;   // runs of rows of the column sums, each a partial row
-
-template <typename T>
-int lna_bwd(const agb::LnaBwdArgs& a, float* dgamma, float* dbeta, int accumulate, float* partial, cudaStream_t st) {
-    agb_int::Device d;
-    AGB_TRY(agb_int::device(&d));
-    const int ub = unit_bytes(addr(a.x) | addr(a.gamma) | addr(a.gy) | addr(a.dx_add) | addr(a.dx), a.hidden * (int)sizeof(T), sizeof(T));
-    const int64_t run = a.rows > 0 ? ceil_div(a.rows, kLnaRuns) : 1;
-    const int runs = static_cast<int>(ceil_div(a.rows, run));
-    const bool columns = dgamma || dbeta;
-    if (columns && runs > 0) {
-        agb::lna_columns<T><<<dim3(static_cast<unsigned>(ceil_div(a.hidden, 256)), runs), 256, 0, st>>>(
-            static_cast<const T*>(a.x), static_cast<const T*>(a.gy), a.mean, a.rstd, partial, a.rows, a.hidden, run);
-        AGB_TRY(after_launch("layernorm_affine_columns"));
+// How the ring kernel takes a call: `upt` units per thread, `block` threads, `ctas` per SM.  stages 0: rows too wide for it.
+struct LnaPlan {
+    int G, block, grid, smem;
+    agb::LnaRing ring;
+};
+LnaPlan plan_lna(int64_t rows, int64_t hidden, int elem, bool whole, int units, int upt, int limit, const agb_int::Device& d) {
+    LnaPlan p{};
+    p.G = threads_per_row(units, upt, limit);
+    if (!p.G) return p;
+    p.block = p.G >= 256 ? p.G : 256 / p.G * p.G;
+    int per_tile = p.block / p.G;
+    const int64_t row_bytes = hidden * elem;
+    // tiles of rows for every SM before tiles of several rows
+    while (per_tile > 1 && ceil_div(rows, per_tile) < d.sms && p.block > 32 && p.G < p.block) {
+        per_tile = (per_tile + 1) / 2;
+        p.block = ceil_div(per_tile * p.G, 32) * 32;
+        per_tile = p.block / p.G;
+        if (p.block == 32) break;
     }
-    if (a.rows > 0)
-        AGB_TRY((ub == 16 ? lna_dx<T, 16>(a, d.sms, st) : ub == 4 ? lna_dx<T, 4>(a, d.sms, st) : lna_dx<T, sizeof(T)>(a, d.sms, st)));
+    const int slack = whole ? 0 : 32;
+    const int64_t tile = ceil_div(per_tile * row_bytes + slack, 128) * 128, sums = per_tile > 1 ? 2 * hidden * 4 : 0;
+    int ctas = limit >= 1024 ? 1024 / p.block : 512 / p.block;          // registers: 64 or 128 a thread
+    if (ctas > kLnaCtas) ctas = kLnaCtas;
+    if (ctas < 1) ctas = 1;
+    int stages = 0;
+    for (; ctas >= 1; --ctas) {
+        int64_t room = d.smem_per_sm / ctas - 1024 - 2048;
+        if (room > d.smem_optin - 2048) room = d.smem_optin - 2048;
+        stages = static_cast<int>(room / (2 * tile));
+        if (stages >= 3 || (ctas == 1 && stages >= 1)) break;
+    }
+    if (ctas < 1) return p;
+    if (stages > 4) stages = 4;
+    p.ring.rows_per_tile = per_tile;
+    p.ring.stages = stages;
+    p.ring.tile_stride = static_cast<int>(tile);
+    p.ring.tiles = ceil_div(rows, per_tile);
+    const int64_t bytes = 2 * tile * stages;
+    p.smem = static_cast<int>(bytes > sums ? bytes : sums);
+    int64_t most = static_cast<int64_t>(d.sms) * ctas;
+    if (most > lna_partials(rows, hidden)) most = lna_partials(rows, hidden);
+    p.grid = static_cast<int>(p.ring.tiles < most ? p.ring.tiles : most);
+    return p;
+}
+
+template <typename T, int UB, int UPT, int MAXT>
+int lna_ring(agb::LnaBwdArgs a, const LnaPlan& p, float* partial, const agb_int::Device& d, cudaStream_t st) {
+    a.G = p.G;
+    AGB_CUDA(cudaFuncSetAttribute(agb::lna_bwd_ring<T, UB, UPT, MAXT>, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem));
+    return launch("layernorm_affine_bwd", agb::lna_bwd_ring<T, UB, UPT, MAXT>, dim3(p.grid), dim3(p.block), p.smem, st, 1, a, p.ring, partial,
+                  d.status);
+}
+
+// The single pass where a row fits a block (32 columns a thread, 512 threads; 8 and 1024 where rows are few and a row's latency counts),
+// else dx and the column sums one after the other.
+template <typename T, int UB>
+int lna_bwd(const agb::LnaBwdArgs& a, float* dgamma, float* dbeta, int accumulate, float* partial, const agb_int::Device& d, cudaStream_t st) {
+    constexpr int N = agb::Unit<T, UB>::N;
+    const bool columns = dgamma || dbeta;
+    int runs = 0;
+    if (a.rows > 0) {
+        LnaPlan p = a.rows <= 2LL * d.sms ? plan_lna(a.rows, a.hidden, sizeof(T), UB == 16, a.hidden / N, 8 / N, 1024, d) : LnaPlan{};
+        const bool few = p.ring.stages > 0;
+        if (!few) p = plan_lna(a.rows, a.hidden, sizeof(T), UB == 16, a.hidden / N, 32 / N, 512, d);
+        if (few) {
+            AGB_TRY((lna_ring<T, UB, 8 / N, 1024>(a, p, columns ? partial : nullptr, d, st)));
+            runs = p.grid;
+        } else if (p.ring.stages > 0) {
+            AGB_TRY((lna_ring<T, UB, 32 / N, 512>(a, p, columns ? partial : nullptr, d, st)));
+            runs = p.grid;
+        } else {
+            const int64_t run = ceil_div(a.rows, kLnaRuns);
+            if (columns) {
+                runs = static_cast<int>(ceil_div(a.rows, run));
+                agb::lna_columns<T><<<dim3(static_cast<unsigned>(ceil_div(a.hidden, 256)), runs), 256, 0, st>>>(
+                    static_cast<const T*>(a.x), static_cast<const T*>(a.gy), a.mean, a.rstd, partial, a.rows, a.hidden, run);
+                AGB_TRY(after_launch("layernorm_affine_columns"));
+            }
+            agb::lna_dx_wide<T, UB><<<static_cast<unsigned>(grid_for(a.rows, 1024, 1024, d.sms, 2)), 1024, 0, st>>>(a);
+            AGB_TRY(after_launch("layernorm_affine_dx"));
+        }
+    }
     if (!columns) return AGB_OK;
-    agb::lna_column_reduce<<<static_cast<unsigned>(ceil_div(2LL * a.hidden, 32)), dim3(32, 8), 0, st>>>(partial, runs, a.hidden, dgamma,
-                                                                                                dbeta, accumulate);
-    return after_launch("layernorm_affine_column_reduce");
+    return launch("layernorm_affine_column_reduce", agb::lna_column_reduce, dim3(static_cast<unsigned>(ceil_div(2LL * a.hidden, 32))), dim3(32, 32), 0,
+                  st, 1, static_cast<const float*>(partial), runs, a.hidden, dgamma, dbeta, accumulate);
 }
 
 // ------------------------------------------------------------------ distillation
@@ -651,9 +710,8 @@ int agb_layernorm_affine_fwd(const void* x, const void* gamma, const void* beta,
 }
 
 size_t agb_layernorm_affine_bwd_workspace_bytes(int64_t rows, int64_t hidden, int dtype) {
-    (void)rows;
     (void)dtype;
-    return hidden <= 0 ? 0 : static_cast<size_t>(kLnaRuns) * 2 * hidden * sizeof(float);
+    return hidden <= 0 ? 0 : static_cast<size_t>(lna_partials(rows, hidden)) * 2 * hidden * sizeof(float);
 }
 
 int agb_layernorm_affine_bwd(const void* x, const void* gamma, const float* mean, const float* rstd, const void* gy, const void* dx_add,
@@ -678,10 +736,15 @@ int agb_layernorm_affine_bwd(const void* x, const void* gamma, const float* mean
         const size_t need = agb_layernorm_affine_bwd_workspace_bytes(rows, hidden, dtype);
         if (workspace_bytes < need) return fail(AGB_ERR_WORKSPACE, "workspace %zu bytes, need %zu", workspace_bytes, need);
     }
+    agb_int::Device d;
+    AGB_TRY(agb_int::device(&d));
     agb::LnaBwdArgs a{x, gamma, mean, rstd, gy, dx_add, dx, rows, static_cast<int>(hidden), 0};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return dtype == AGB_F32 ? lna_bwd<float>(a, dgamma, dbeta, accumulate, static_cast<float*>(workspace), st)
-                            : lna_bwd<bf16>(a, dgamma, dbeta, accumulate, static_cast<float*>(workspace), st);
+    float* part = static_cast<float*>(workspace);
+    const int ub = unit_bytes(addr(x) | addr(gamma) | addr(gy) | addr(dx_add) | addr(dx), hidden * elem, elem);
+    if (dtype == AGB_F32)
+        return ub == 16 ? lna_bwd<float, 16>(a, dgamma, dbeta, accumulate, part, d, st) : lna_bwd<float, 4>(a, dgamma, dbeta, accumulate, part, d, st);
+    return ub == 16 ? lna_bwd<bf16, 16>(a, dgamma, dbeta, accumulate, part, d, st) : lna_bwd<bf16, 2>(a, dgamma, dbeta, accumulate, part, d, st);
 }
 
 int agb_distill_topk_fwd(const void* z, const void* idx, int idx_type, const void* teacher, int teacher_dtype, float* loss, float* lse,

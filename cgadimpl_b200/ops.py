@@ -216,39 +216,59 @@ def layernorm_jvp(y, t, var, eps=1e-5, out=None):
     return ty
 
 
-def _on(t):
-    """Makes t's device the current one (the library launches on the current device and its current stream)."""
-    return torch.cuda.device(t.device)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
+def _call(like, fn, *args):
+    """fn(*args, stream) on like's device and its current stream, checked.  These wrappers sit in front of kernels of a few
+    microseconds: the device is only switched where it has to be, and pointers go to ctypes as integers."""
+    dev = like.get_device()
+    if dev == _current_device():
+        status = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, _raw_stream(dev))
+    if status:
+        check(status)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _out(t, shape, dtype, like, name):
     """The caller's output tensor, checked, or a new one on like's device."""
     if t is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
+        return like.new_empty(shape, dtype=dtype)
     if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != like.device or not t.is_contiguous():
         raise ValueError(f"{name} {tuple(t.shape)} {t.dtype} on {t.device}: expected contiguous {tuple(shape)} {dtype} on {like.device}")
     return t
 
 
 def _workspace(t, nbytes, like):
+    """(address, bytes, the tensor that holds them) of the caller's workspace, checked, or of a new one."""
     if t is None:
-        return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+        t = like.new_empty((nbytes,), dtype=torch.uint8)
+        return t.data_ptr(), nbytes, t
     if t.device != like.device or not t.is_contiguous():
         raise ValueError(f"workspace on {t.device}: expected a contiguous tensor on {like.device}")
-    return t
+    return t.data_ptr(), t.numel() * t.element_size(), t
 
 
 def layernorm_affine_fwd(x, gamma, beta=None, eps=1e-5, out=None, mean=None, rstd=None):
     """y = (x - mean) * rstd * gamma + beta; returns (y, mean[rows], rstd[rows]), the statistics in fp32."""
     rows, hidden = _rows_hidden(x)
-    with _on(x):
-        y = torch.empty_like(x) if out is None else out
-        mean, rstd = _out(mean, (rows,), torch.float32, x, "mean"), _out(rstd, (rows,), torch.float32, x, "rstd")
-        _same(x, y)
-        _vec(x, hidden, x.dtype, gamma, beta)
-        check(_lib.lib().agb_layernorm_affine_fwd(_p(x), _p(gamma), _p(beta), _p(y), _p(mean), _p(rstd), rows, hidden, eps, _dt(x),
-                                                  _stream()))
-    return y, mean, rstd
+    dt = _dt(x)
+    _vec(x, hidden, x.dtype, gamma, beta)
+    if out is None:
+        out = torch.empty_like(x)
+    else:
+        _same(x, out)
+    mean, rstd = _out(mean, (rows,), torch.float32, x, "mean"), _out(rstd, (rows,), torch.float32, x, "rstd")
+    _call(x, _lib.lib().agb_layernorm_affine_fwd, x.data_ptr(), gamma.data_ptr(), _ptr(beta), out.data_ptr(), mean.data_ptr(),
+          rstd.data_ptr(), rows, hidden, eps, dt)
+    return out, mean, rstd
 
 
 def layernorm_affine_bwd(x, gamma, mean, rstd, gy, dx_add=None, dx=None, dgamma=None, dbeta=None, accumulate=False, with_beta=True,
@@ -260,17 +280,20 @@ def layernorm_affine_bwd(x, gamma, mean, rstd, gy, dx_add=None, dx=None, dgamma=
         raise ValueError("accumulate needs the tensors to add to")
     if dbeta is not None and not with_beta:
         raise ValueError("dbeta given with with_beta=False")
-    with _on(x):
-        dx = torch.empty_like(x) if dx is None else dx
-        dgamma = _out(dgamma, (hidden,), torch.float32, x, "dgamma")
-        dbeta = _out(dbeta, (hidden,), torch.float32, x, "dbeta") if with_beta else None
-        _same(x, gy, dx_add, dx)
-        _vec(x, hidden, x.dtype, gamma)
-        _vec(x, rows, torch.float32, mean, rstd)
-        ws = _workspace(workspace, _lib.lib().agb_layernorm_affine_bwd_workspace_bytes(rows, hidden, _dt(x)), x)
-        check(_lib.lib().agb_layernorm_affine_bwd(_p(x), _p(gamma), _p(mean), _p(rstd), _p(gy), _p(dx_add), _p(dx), _p(dgamma), _p(dbeta),
-                                                  int(bool(accumulate)), _p(ws), ws.numel() * ws.element_size(), rows, hidden, _dt(x),
-                                                  _stream()))
+    dt = _dt(x)
+    _same(x, gy, dx_add)
+    _vec(x, hidden, x.dtype, gamma)
+    _vec(x, rows, torch.float32, mean, rstd)
+    if dx is None:
+        dx = torch.empty_like(x)
+    else:
+        _same(x, dx)
+    dgamma = _out(dgamma, (hidden,), torch.float32, x, "dgamma")
+    dbeta = _out(dbeta, (hidden,), torch.float32, x, "dbeta") if with_beta else None
+    lib = _lib.lib()
+    ws, nbytes, keep = _workspace(workspace, lib.agb_layernorm_affine_bwd_workspace_bytes(rows, hidden, dt), x)
+    _call(x, lib.agb_layernorm_affine_bwd, x.data_ptr(), gamma.data_ptr(), mean.data_ptr(), rstd.data_ptr(), gy.data_ptr(), _ptr(dx_add),
+          dx.data_ptr(), dgamma.data_ptr(), _ptr(dbeta), int(bool(accumulate)), ws, nbytes, rows, hidden, dt)
     return dx, dgamma, dbeta
 
 
@@ -293,15 +316,24 @@ def _ce_operands(h, w, target):
     return rows, hidden, w.shape[0]
 
 
+def _ce_bytes(h, backward, rows, hidden, vocab, dt):
+    """The workspace's size depends on the device: asked on h's."""
+    fn, dev = _lib.lib().agb_linear_ce_workspace_bytes, h.get_device()
+    if dev == _current_device():
+        return fn(backward, rows, hidden, vocab, dt)
+    with torch.cuda.device(dev):
+        return fn(backward, rows, hidden, vocab, dt)
+
+
 def linear_ce_fwd(h, w, target, loss=None, lse=None, workspace=None):
     """Cross entropy of softmax(h w') against target (int32 or int64), the logits not kept; returns (loss[rows], lse[rows]) in fp32.
     Rows whose target lies outside [0, vocab) take no part: loss = lse = 0."""
     rows, hidden, vocab = _ce_operands(h, w, target)
-    with _on(h):
-        loss, lse = _out(loss, (rows,), torch.float32, h, "loss"), _out(lse, (rows,), torch.float32, h, "lse")
-        ws = _workspace(workspace, _lib.lib().agb_linear_ce_workspace_bytes(0, rows, hidden, vocab, _dt(h)), h)
-        check(_lib.lib().agb_linear_ce_fwd(_p(h), _p(w), _p(target), _it(target, "target"), _p(loss), _p(lse), rows, hidden, vocab, _dt(h),
-                                           _p(ws), ws.numel() * ws.element_size(), _stream()))
+    dt, it = _dt(h), _it(target, "target")
+    loss, lse = _out(loss, (rows,), torch.float32, h, "loss"), _out(lse, (rows,), torch.float32, h, "lse")
+    ws, nbytes, keep = _workspace(workspace, _ce_bytes(h, 0, rows, hidden, vocab, dt) if workspace is None else 0, h)
+    _call(h, _lib.lib().agb_linear_ce_fwd, h.data_ptr(), w.data_ptr(), target.data_ptr(), it, loss.data_ptr(), lse.data_ptr(), rows, hidden,
+          vocab, dt, ws, nbytes)
     return loss, lse
 
 
@@ -310,16 +342,15 @@ def linear_ce_bwd(h, w, target, lse, gy, dh=None, dw=None, accumulate_dw=False, 
     rows, hidden, vocab = _ce_operands(h, w, target)
     if accumulate_dw and dw is None:
         raise ValueError("accumulate_dw needs the dw to add to")
-    with _on(h):
-        dh = (torch.empty_like(h) if dh is None else dh) if need_dh else None
-        dw = (torch.empty_like(w) if dw is None else dw) if need_dw else None
-        _same(h, dh)
-        _same(w, dw)
-        _vec(h, rows, torch.float32, lse, gy)
-        ws = _workspace(workspace, _lib.lib().agb_linear_ce_workspace_bytes(1, rows, hidden, vocab, _dt(h)), h)
-        check(_lib.lib().agb_linear_ce_bwd(_p(h), _p(w), _p(target), _it(target, "target"), _p(lse), _p(gy), _p(dh), _p(dw),
-                                           int(bool(accumulate_dw)), rows, hidden, vocab, _dt(h), _p(ws), ws.numel() * ws.element_size(),
-                                           _stream()))
+    dt, it = _dt(h), _it(target, "target")
+    dh = (torch.empty_like(h) if dh is None else dh) if need_dh else None
+    dw = (torch.empty_like(w) if dw is None else dw) if need_dw else None
+    _same(h, dh)
+    _same(w, dw)
+    _vec(h, rows, torch.float32, lse, gy)
+    ws, nbytes, keep = _workspace(workspace, _ce_bytes(h, 1, rows, hidden, vocab, dt) if workspace is None else 0, h)
+    _call(h, _lib.lib().agb_linear_ce_bwd, h.data_ptr(), w.data_ptr(), target.data_ptr(), it, lse.data_ptr(), gy.data_ptr(), _ptr(dh), _ptr(dw),
+          int(bool(accumulate_dw)), rows, hidden, vocab, dt, ws, nbytes)
     return dh, dw
 
 
@@ -339,35 +370,35 @@ def distill_topk_fwd(z, idx, teacher, temperature=1.0, loss=None, lse=None):
     temperature^2 * KL(softmax_k(teacher / t) || softmax(z / t)); returns (loss[rows], lse[rows]) in fp32.  Entries whose index
     lies outside [0, vocab) take no part; a row without entries has loss = lse = 0."""
     rows, vocab, k = _distill_operands(z, idx, teacher)
-    with _on(z):
-        loss, lse = _out(loss, (rows,), torch.float32, z, "loss"), _out(lse, (rows,), torch.float32, z, "lse")
-        check(_lib.lib().agb_distill_topk_fwd(_p(z), _p(idx), _it(idx, "idx"), _p(teacher), _dt(teacher), _p(loss), _p(lse), rows, vocab,
-                                              k, temperature, _dt(z), _stream()))
+    dt, it, tt = _dt(z), _it(idx, "idx"), _dt(teacher)
+    loss, lse = _out(loss, (rows,), torch.float32, z, "loss"), _out(lse, (rows,), torch.float32, z, "lse")
+    _call(z, _lib.lib().agb_distill_topk_fwd, z.data_ptr(), idx.data_ptr(), it, teacher.data_ptr(), tt, loss.data_ptr(), lse.data_ptr(), rows,
+          vocab, k, temperature, dt)
     return loss, lse
 
 
 def distill_topk_bwd(z, idx, teacher, lse, gy, temperature=1.0, dz_add=None, dz=None):
     """dz = gy[rows] * t * (softmax(z / t) - the teacher's shares) [+ dz_add], lse from distill_topk_fwd."""
     rows, vocab, k = _distill_operands(z, idx, teacher)
-    with _on(z):
-        dz = torch.empty_like(z) if dz is None else dz
-        _same(z, dz_add, dz)
-        _vec(z, rows, torch.float32, lse, gy)
-        check(_lib.lib().agb_distill_topk_bwd(_p(z), _p(idx), _it(idx, "idx"), _p(teacher), _dt(teacher), _p(lse), _p(gy), _p(dz_add),
-                                              _p(dz), rows, vocab, k, temperature, _dt(z), _stream()))
+    dt, it, tt = _dt(z), _it(idx, "idx"), _dt(teacher)
+    dz = torch.empty_like(z) if dz is None else dz
+    _same(z, dz_add, dz)
+    _vec(z, rows, torch.float32, lse, gy)
+    _call(z, _lib.lib().agb_distill_topk_bwd, z.data_ptr(), idx.data_ptr(), it, teacher.data_ptr(), tt, lse.data_ptr(), gy.data_ptr(),
+          _ptr(dz_add), dz.data_ptr(), rows, vocab, k, temperature, dt)
     return dz
 
 
 def distill_topk_fwd_bwd(z, idx, teacher, gy, temperature=1.0, dz_add=None, loss=None, lse=None, dz=None):
     """Both in one pass over the logits, for a gy known beforehand; returns (loss, lse, dz).  dz may be z itself."""
     rows, vocab, k = _distill_operands(z, idx, teacher)
-    with _on(z):
-        loss, lse = _out(loss, (rows,), torch.float32, z, "loss"), _out(lse, (rows,), torch.float32, z, "lse")
-        dz = torch.empty_like(z) if dz is None else dz
-        _same(z, dz_add, dz)
-        _vec(z, rows, torch.float32, gy)
-        check(_lib.lib().agb_distill_topk_fwd_bwd(_p(z), _p(idx), _it(idx, "idx"), _p(teacher), _dt(teacher), _p(gy), _p(dz_add), _p(loss),
-                                                  _p(lse), _p(dz), rows, vocab, k, temperature, _dt(z), _stream()))
+    dt, it, tt = _dt(z), _it(idx, "idx"), _dt(teacher)
+    loss, lse = _out(loss, (rows,), torch.float32, z, "loss"), _out(lse, (rows,), torch.float32, z, "lse")
+    dz = torch.empty_like(z) if dz is None else dz
+    _same(z, dz_add, dz)
+    _vec(z, rows, torch.float32, gy)
+    _call(z, _lib.lib().agb_distill_topk_fwd_bwd, z.data_ptr(), idx.data_ptr(), it, teacher.data_ptr(), tt, gy.data_ptr(), _ptr(dz_add),
+          loss.data_ptr(), lse.data_ptr(), dz.data_ptr(), rows, vocab, k, temperature, dt)
     return loss, lse, dz
 
 
