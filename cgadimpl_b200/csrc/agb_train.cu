@@ -80,33 +80,19 @@ inline int unit_bytes(uintptr_t all, int64_t row_bytes, int elem) {
     return m % 16 == 0 ? 16 : (m % 4 == 0 ? 4 : elem);
 }
 
-// Threads per row for `units` units at `upt` per thread: a power of two up to a warp, else whole warps; 0: too many.
+// Threads per row for `units` units at `upt` per thread: a power of two up to a warp (one unit each), else whole warps; 0: too many.
 inline int threads_per_row(int64_t units, int upt, int limit) {
-    const int64_t want = ceil_div(units, upt);
-    if (want <= 32) {
+    if (units <= 32 && upt == 1) {
         int g = 1;
-        while (g < want) g *= 2;
+        while (g < units) g *= 2;
         return g;
     }
-    const int64_t g = ceil_div(want, 32) * 32;
+    const int64_t g = ceil_div(units, 32LL * upt) * 32;
     return g > limit ? 0 : static_cast<int>(g);
 }
 inline int64_t grid_for(int64_t rows, int G, int block, int sms, int per_sm) {
     const int64_t want = ceil_div(rows, G <= 32 ? block / G : 1), cap = static_cast<int64_t>(sms) * per_sm;
     return want < cap ? want : cap;
-}
-
-template <typename T, int UB>
-int lna_fwd(agb::LnaFwdArgs a, int sms, cudaStream_t st) {
-    constexpr int N = agb::Unit<T, UB>::N, UPT = 32 / N;
-    a.G = threads_per_row(a.hidden / N, UPT, 512);
-    if (a.G) {
-        const int block = a.G <= 32 ? 128 : a.G;
-        agb::lna_fwd_kernel<T, UB, UPT><<<static_cast<unsigned>(grid_for(a.rows, a.G, block, sms, 2048 / block)), block, 0, st>>>(a);
-    } else {
-        agb::lna_fwd_wide<T, UB><<<static_cast<unsigned>(grid_for(a.rows, 1024, 1024, sms, 2)), 1024, 0, st>>>(a);
-    }
-    return after_launch("layernorm_affine_fwd");
 }
 
 constexpr int kLnaRuns = 64;        // wide rows: runs of rows of the column sums, each a partial row
@@ -122,7 +108,18 @@ struct LnaPlan {
     int G, block, grid, smem;
     agb::LnaRing ring;
 };
-LnaPlan plan_lna(int64_t rows, int64_t hidden, int elem, bool whole, int units, int upt, int limit, const agb_int::Device& d) {
+// Columns a thread takes: one unit where a row has no more than a warp's worth of them; eight where rows are few and a row's latency
+// counts (the threads of a row then add up to 1024), and in the backward of rows that are taken element by element, whose instructions and
+// not the sums' registers are the limit (8192 x 2047 fp32: 47 us with eight, 64 us with 32; 4099 x 1001 bf16: 18 and 34 us); else 32, which
+// spreads the fixed cost of a row over more columns (32768 x 4096 bf16: 149 us with 32, 281 us with eight).
+enum LnaWidth { kLnaUnit = 0, kLnaEight = 1, kLnaWide = 2 };
+LnaWidth lna_width(int64_t rows, int64_t units, int n, bool backward, int sms) {
+    if (units <= 32) return kLnaUnit;
+    return units * n <= 8192 && (rows <= 2LL * sms || (backward && n == 1)) ? kLnaEight : kLnaWide;
+}
+
+// `arrays`: 1 forward, 2 backward.
+LnaPlan plan_lna(int64_t rows, int64_t hidden, int elem, bool whole, int64_t units, int upt, int limit, int arrays, const agb_int::Device& d) {
     LnaPlan p{};
     p.G = threads_per_row(units, upt, limit);
     if (!p.G) return p;
@@ -137,15 +134,15 @@ LnaPlan plan_lna(int64_t rows, int64_t hidden, int elem, bool whole, int units, 
         if (p.block == 32) break;
     }
     const int slack = whole ? 0 : 32;
-    const int64_t tile = ceil_div(per_tile * row_bytes + slack, 128) * 128, sums = per_tile > 1 ? 2 * hidden * 4 : 0;
-    int ctas = limit >= 1024 ? 1024 / p.block : 512 / p.block;          // registers: 64 or 128 a thread
+    const int64_t tile = ceil_div(per_tile * row_bytes + slack, 128) * 128, sums = arrays == 2 && per_tile > 1 ? 2 * hidden * 4 : 0;
+    int ctas = (limit >= 1024 || upt == 1 ? 1024 : 512) / p.block;          // registers: 64 or 128 a thread
     if (ctas > kLnaCtas) ctas = kLnaCtas;
     if (ctas < 1) ctas = 1;
     int stages = 0;
     for (; ctas >= 1; --ctas) {
         int64_t room = d.smem_per_sm / ctas - 1024 - 2048;
         if (room > d.smem_optin - 2048) room = d.smem_optin - 2048;
-        stages = static_cast<int>(room / (2 * tile));
+        stages = static_cast<int>(room / (arrays * tile));
         if (stages >= 3 || (ctas == 1 && stages >= 1)) break;
     }
     if (ctas < 1) return p;
@@ -154,12 +151,34 @@ LnaPlan plan_lna(int64_t rows, int64_t hidden, int elem, bool whole, int units, 
     p.ring.stages = stages;
     p.ring.tile_stride = static_cast<int>(tile);
     p.ring.tiles = ceil_div(rows, per_tile);
-    const int64_t bytes = 2 * tile * stages;
+    const int64_t bytes = arrays * tile * stages;
     p.smem = static_cast<int>(bytes > sums ? bytes : sums);
     int64_t most = static_cast<int64_t>(d.sms) * ctas;
-    if (most > lna_partials(rows, hidden)) most = lna_partials(rows, hidden);
+    if (arrays == 2 && most > lna_partials(rows, hidden)) most = lna_partials(rows, hidden);
     p.grid = static_cast<int>(p.ring.tiles < most ? p.ring.tiles : most);
     return p;
+}
+
+template <typename T, int UB, int UPT, int MAXT>
+int lna_fwd_launch(agb::LnaFwdArgs a, const LnaPlan& p, const agb_int::Device& d, cudaStream_t st) {
+    a.G = p.G;
+    AGB_CUDA(cudaFuncSetAttribute(agb::lna_fwd_ring<T, UB, UPT, MAXT>, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem));
+    return launch("layernorm_affine_fwd", agb::lna_fwd_ring<T, UB, UPT, MAXT>, dim3(p.grid), dim3(p.block), p.smem, st, 1, a, p.ring, d.status);
+}
+template <typename T, int UB>
+int lna_fwd(const agb::LnaFwdArgs& a, const agb_int::Device& d, cudaStream_t st) {
+    constexpr int N = agb::Unit<T, UB>::N;
+    const int64_t units = a.hidden / N;
+    auto plan = [&](int upt, int limit) { return plan_lna(a.rows, a.hidden, sizeof(T), UB == 16, units, upt, limit, 1, d); };
+    const LnaWidth width = lna_width(a.rows, units, N, false, d.sms);
+    LnaPlan p = width == kLnaUnit ? plan(1, 512) : width == kLnaEight ? plan(8 / N, 1024) : plan(32 / N, 512);
+    if (p.ring.stages > 0) {
+        if (width == kLnaUnit) return lna_fwd_launch<T, UB, 1, 512>(a, p, d, st);
+        if (width == kLnaEight) return lna_fwd_launch<T, UB, 8 / N, 1024>(a, p, d, st);
+        return lna_fwd_launch<T, UB, 32 / N, 512>(a, p, d, st);
+    }
+    agb::lna_fwd_wide<T, UB><<<static_cast<unsigned>(grid_for(a.rows, 1024, 1024, d.sms, 2)), 1024, 0, st>>>(a);
+    return after_launch("layernorm_affine_fwd");
 }
 
 template <typename T, int UB, int UPT, int MAXT>
@@ -178,15 +197,16 @@ int lna_bwd(const agb::LnaBwdArgs& a, float* dgamma, float* dbeta, int accumulat
     const bool columns = dgamma || dbeta;
     int runs = 0;
     if (a.rows > 0) {
-        LnaPlan p = a.rows <= 2LL * d.sms ? plan_lna(a.rows, a.hidden, sizeof(T), UB == 16, a.hidden / N, 8 / N, 1024, d) : LnaPlan{};
-        const bool few = p.ring.stages > 0;
-        if (!few) p = plan_lna(a.rows, a.hidden, sizeof(T), UB == 16, a.hidden / N, 32 / N, 512, d);
-        if (few) {
-            AGB_TRY((lna_ring<T, UB, 8 / N, 1024>(a, p, columns ? partial : nullptr, d, st)));
+        const int64_t units = a.hidden / N;
+        auto plan = [&](int upt, int limit) { return plan_lna(a.rows, a.hidden, sizeof(T), UB == 16, units, upt, limit, 2, d); };
+        const LnaWidth width = lna_width(a.rows, units, N, true, d.sms);
+        const LnaPlan p = width == kLnaUnit ? plan(1, 512) : width == kLnaEight ? plan(8 / N, 1024) : plan(32 / N, 512);
+        float* to = columns ? partial : nullptr;
+        if (p.ring.stages > 0) {
             runs = p.grid;
-        } else if (p.ring.stages > 0) {
-            AGB_TRY((lna_ring<T, UB, 32 / N, 512>(a, p, columns ? partial : nullptr, d, st)));
-            runs = p.grid;
+            if (width == kLnaUnit) AGB_TRY((lna_ring<T, UB, 1, 512>(a, p, to, d, st)));
+            else if (width == kLnaEight) AGB_TRY((lna_ring<T, UB, 8 / N, 1024>(a, p, to, d, st)));
+            else AGB_TRY((lna_ring<T, UB, 32 / N, 512>(a, p, to, d, st)));
         } else {
             const int64_t run = ceil_div(a.rows, kLnaRuns);
             if (columns) {
@@ -705,8 +725,8 @@ int agb_layernorm_affine_fwd(const void* x, const void* gamma, const void* beta,
     agb::LnaFwdArgs a{x, gamma, beta, y, mean, rstd, rows, static_cast<int>(hidden), 0, eps};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int ub = unit_bytes(addr(x) | addr(gamma) | addr(beta) | addr(y), hidden * elem, elem);
-    if (dtype == AGB_F32) return ub == 16 ? lna_fwd<float, 16>(a, d.sms, st) : lna_fwd<float, 4>(a, d.sms, st);
-    return ub == 16 ? lna_fwd<bf16, 16>(a, d.sms, st) : ub == 4 ? lna_fwd<bf16, 4>(a, d.sms, st) : lna_fwd<bf16, 2>(a, d.sms, st);
+    if (dtype == AGB_F32) return ub == 16 ? lna_fwd<float, 16>(a, d, st) : lna_fwd<float, 4>(a, d, st);
+    return ub == 16 ? lna_fwd<bf16, 16>(a, d, st) : lna_fwd<bf16, 2>(a, d, st);
 }
 
 size_t agb_layernorm_affine_bwd_workspace_bytes(int64_t rows, int64_t hidden, int dtype) {

@@ -6,6 +6,8 @@
 // the centred values (a second pass over registers), so an offset of the row costs no digits.
 // No contraction of a size that matters: bound by memory.
 #pragma once
+#include <type_traits>
+
 #include "agb_device.cuh"
 
 namespace agb {
@@ -65,6 +67,49 @@ struct Unit<__nv_bfloat16, 2> {
     __device__ __forceinline__ static raw pack(const float* f) { return __bfloat16_as_ushort(__float2bfloat16_rn(f[0])); }
 };
 
+// Two lanes of fp32 at once (one instruction each on sm_100a).
+__device__ __forceinline__ float2 pk(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 fma2p(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+// A thread's UPT units of a row as pairs of fp32 (a unit of one element shares a pair with the next unit).  The units lie 32 apart, so
+// that a warp reads neighbours and every offset is a constant of the instruction.  Units at or behind `lim` do not exist: they load as
+// zeros and are not stored; FULL says that there are none.
+template <typename T, int UB, int UPT>
+struct Slice {
+    typedef Unit<T, UB> U;
+    typedef typename U::raw raw;
+    static constexpr int N = U::N, NV = UPT * N, P = (NV + 1) / 2;
+    template <bool FULL, typename L>
+    __device__ __forceinline__ static void load(float2 (&f)[P], int lim, L get) {
+        float v[2 * P];
+        v[2 * P - 1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < UPT; ++i) {
+            raw u{};
+            if (FULL || 32 * i < lim) u = get(32 * i);
+            U::unpack(u, v + i * N);
+        }
+#pragma unroll
+        for (int e = 0; e < P; ++e) f[e] = make_float2(v[2 * e], v[2 * e + 1]);
+    }
+    template <bool FULL, typename F>
+    __device__ __forceinline__ static void store(const float2 (&f)[P], int lim, F put) {
+        float v[2 * P];
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+            v[2 * e] = f[e].x;
+            v[2 * e + 1] = f[e].y;
+        }
+#pragma unroll
+        for (int i = 0; i < UPT; ++i)
+            if (FULL || 32 * i < lim) put(32 * i, U::pack(v + i * N));
+    }
+    __device__ __forceinline__ static float at(const float2 (&f)[P], int e) { return e & 1 ? f[e >> 1].y : f[e >> 1].x; }
+};
+// First unit of thread t of a row of G threads (G below 32: one unit per thread).
+__device__ __forceinline__ int first_unit(int t, int G, int upt) { return G <= 32 ? t : (t >> 5) * 32 * upt + (t & 31); }
+
 // Sum over the G threads of a row, the same bits in each of them.  G is a power of two up to 32 (parts of a warp; several rows
 // to a warp) or the whole block.  `scratch`: one float per warp, reused after the second barrier.
 __device__ __forceinline__ float row_sum(float v, int G, float* scratch) {
@@ -89,67 +134,150 @@ struct LnaFwdArgs {
     float eps;
 };
 
-// One row per G threads, UPT units per thread held in registers between the two passes.
-template <typename T, int UB, int UPT>
-__global__ void __launch_bounds__(512) lna_fwd_kernel(const LnaFwdArgs a) {
-    typedef Unit<T, UB> U;
-    typedef typename U::raw raw;
-    __shared__ float scratch[32];
-    const int G = a.G, t = threadIdx.x & (G <= 32 ? G - 1 : 1023);
-    const int per_block = blockDim.x / G, nunits = a.hidden / U::N;
-    const float inv_h = __fdiv_rn(1.f, static_cast<float>(a.hidden));
-    const int64_t stride = static_cast<int64_t>(gridDim.x) * per_block;
-    const int64_t groups = (a.rows + per_block - 1) / per_block * per_block;   // whole warps take every turn (shuffles)
-    for (int64_t r = static_cast<int64_t>(blockIdx.x) * per_block + (G <= 32 ? threadIdx.x / G : 0); r < groups; r += stride) {
+struct LnaRing {
+    int rows_per_tile, stages, tile_stride;    // bytes of a tile's slot for one array
+    int64_t tiles;
+};
+
+// Copies a tile's bytes [at, at + bytes) of a tensor of `total` bytes into a slot.
+template <bool WHOLE>
+__device__ __forceinline__ void lna_copy(uint8_t* slot, const uint8_t* base, int64_t at, int bytes, int64_t total, uint64_t* bar, int elem) {
+    if (WHOLE) {
+        bulk_load(slot, base + at, bytes, bar);
+        return;
+    }
+    const uint8_t* p = base + at;
+    const int lead = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15);
+    int lo = -lead, hi = (lead + bytes + 15) / 16 * 16 - lead;                 // relative to p
+    if (at + lo < 0) lo += 16;
+    if (at + hi > total) hi -= 16;
+    // the ends of the tensor, at most 15 bytes each (and the whole of a tile of a few bytes)
+    const int head = lo < 0 ? 0 : (lo < bytes ? lo : bytes);
+    for (int i = 0; i < head; i += elem)
+        for (int b = 0; b < elem; b += 2) *reinterpret_cast<uint16_t*>(slot + lead + i + b) = *reinterpret_cast<const uint16_t*>(p + i + b);
+    for (int i = hi > head ? hi : head; i < bytes; i += elem)
+        for (int b = 0; b < elem; b += 2) *reinterpret_cast<uint16_t*>(slot + lead + i + b) = *reinterpret_cast<const uint16_t*>(p + i + b);
+    mbar_arrive_expect_tx(bar, hi > lo ? hi - lo : 0);
+    if (hi > lo) bulk_load(slot + lead + lo, p + lo, hi - lo, bar);
+}
+
+
+// Forward.  The ring of lna_bwd_ring with one array; a thread takes its slice of the row out of the tile into registers, and the mean and
+// the centred squares are summed from there.  Two block barriers per tile where a row is several warps, the first of which also frees
+// the slot.
+template <typename T, int UB, int UPT, int MAXT>
+__global__ void __launch_bounds__(MAXT) lna_fwd_ring(const LnaFwdArgs a, const LnaRing g, int* status) {
+    typedef Slice<T, UB, UPT> L;
+    typedef typename L::raw raw;
+    constexpr int N = L::N, P = L::P, S = 8;
+    constexpr bool WHOLE = UB == 16;
+    extern __shared__ __align__(128) uint8_t lna_smem[];
+    __shared__ __align__(8) uint64_t full[S];
+    __shared__ float scratch[2][32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int G = a.G, t = tid % G, mine = tid / G;
+    const int H = a.hidden, first = first_unit(t, G, UPT), lim = H / N - first;
+    const bool all = __all_sync(0xffffffffu, lim > 32 * (UPT - 1));
+    const int64_t row_bytes = static_cast<int64_t>(H) * sizeof(T), total = a.rows * row_bytes;
+    const uint8_t* xb = static_cast<const uint8_t*>(a.x);
+    if (tid == 0) {
+        for (int s = 0; s < g.stages; ++s) mbar_init(&full[s], 1);
+        mbar_fence_init();
+    }
+    __syncthreads();
+    pdl_wait();
+    pdl_trigger();
+    auto issue = [&](int64_t k, int s) {
+        const int64_t r0 = k * g.rows_per_tile;
+        const int rows = static_cast<int>(a.rows - r0 < g.rows_per_tile ? a.rows - r0 : g.rows_per_tile);
+        const int bytes = static_cast<int>(rows * row_bytes);
+        if (WHOLE) mbar_arrive_expect_tx(&full[s], bytes);
+        lna_copy<WHOLE>(lna_smem + static_cast<int64_t>(s) * g.tile_stride, xb, r0 * row_bytes, bytes, total, &full[s], sizeof(T));
+    };
+    const int64_t step = gridDim.x;
+    if (tid == 0) {
+        int64_t k = blockIdx.x;
+        for (int s = 0; s < g.stages && k < g.tiles; ++s, k += step) issue(k, s);
+    }
+    const raw* gamma = reinterpret_cast<const raw*>(a.gamma) + first;
+    const raw* beta = reinterpret_cast<const raw*>(a.beta) + first;
+    const bool with_beta = a.beta != nullptr;
+    const float inv_h = __fdiv_rn(1.f, static_cast<float>(H));
+    const int w0 = mine * (G >> 5), w1 = w0 + (G >> 5);
+    // sum over the row's threads; the scratch of the two sums of a tile alternates, so that one barrier each is enough
+    auto row_total = [&](float v, int which) {
+        for (int o = (G < 32 ? G : 32) >> 1; o > 0; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, o));
+        if (G <= 32) return v;
+        if (lane == 0) scratch[which][warp] = v;
+        __syncthreads();
+        v = 0.f;
+        for (int w = w0; w < w1; w += 4) {             // four loads in flight
+            float q[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) q[u] = w + u < w1 ? scratch[which][w + u] : 0.f;
+            v = __fadd_rn(v, __fadd_rn(__fadd_rn(q[0], q[1]), __fadd_rn(q[2], q[3])));
+        }
+        return v;
+    };
+    int s = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    auto tile = [&](auto full_tag, int64_t k) {
+        constexpr bool FULL = decltype(full_tag)::value;
+        const int64_t r = k * g.rows_per_tile + mine;
         const bool live = r < a.rows;
-        const raw* x = reinterpret_cast<const raw*>(static_cast<const T*>(a.x) + r * a.hidden);
-        float f[UPT][U::N];
-        float s = 0.f;
-        raw u[UPT];
+        const int n = live ? lim : 0;
+        const int ox = WHOLE ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(xb + k * g.rows_per_tile * row_bytes) & 15);
+        const raw* x = reinterpret_cast<const raw*>(lna_smem + static_cast<int64_t>(s) * g.tile_stride + ox + mine * row_bytes) + first;
+        float2 f[P];
+        L::template load<FULL>(f, n, [&](int u) { return x[u]; });
+        float2 v = f[0];
 #pragma unroll
-        for (int i = 0; i < UPT; ++i)
-            if (live && t + i * G < nunits) u[i] = x[t + i * G];
+        for (int e = 1; e < P; ++e) v = add2(v, f[e]);
+        if (G <= 32) __syncthreads();                  // everyone has taken the tile out of its slot
+        const float mean = __fmul_rn(row_total(__fadd_rn(v.x, v.y), 0), inv_h);
+        if (tid == 0 && k + g.stages * step < g.tiles) issue(k + g.stages * step, s);      // row_total's barrier has been passed
+        v = pk(0.f);
 #pragma unroll
-        for (int i = 0; i < UPT; ++i)
-            if (live && t + i * G < nunits) {
-                U::unpack(u[i], f[i]);
-#pragma unroll
-                for (int e = 0; e < U::N; ++e) s = __fadd_rn(s, f[i][e]);
-            }
-        const float mean = __fmul_rn(row_sum(s, G, scratch), inv_h);
-        s = 0.f;
-#pragma unroll
-        for (int i = 0; i < UPT; ++i)
-            if (live && t + i * G < nunits) {
-#pragma unroll
-                for (int e = 0; e < U::N; ++e) {
-                    f[i][e] = __fsub_rn(f[i][e], mean);
-                    s = __fmaf_rn(f[i][e], f[i][e], s);
-                }
-            }
-        const float rstd = __fdiv_rn(1.f, __fsqrt_rn(__fmaf_rn(row_sum(s, G, scratch), inv_h, a.eps)));
-        if (!live) continue;
-        if (t == 0) {
+        for (int e = 0; e < P; ++e) {
+            // columns that do not exist add nothing to the squares
+            const bool x0 = FULL && 2 * e < L::NV ? true : 32 * (2 * e / N) < n, x1 = (2 * e + 1 < L::NV) && (FULL || 32 * ((2 * e + 1) / N) < n);
+            f[e] = add2(f[e], make_float2(x0 ? -mean : 0.f, x1 ? -mean : 0.f));
+            v = fma2p(f[e], f[e], v);
+        }
+        const float rstd = rsqrtf(__fmaf_rn(row_total(__fadd_rn(v.x, v.y), 1), inv_h, a.eps));
+        if (live && t == 0) {
             a.mean[r] = mean;
             a.rstd[r] = rstd;
         }
-        raw* y = reinterpret_cast<raw*>(static_cast<T*>(a.y) + r * a.hidden);
-        const raw* gamma = reinterpret_cast<const raw*>(a.gamma);
-        const raw* beta = reinterpret_cast<const raw*>(a.beta);
+        raw* y = reinterpret_cast<raw*>(static_cast<T*>(a.y) + r * H) + first;
+        float2 w[P];
+        L::template load<FULL>(w, n, [&](int u) { return __ldg(gamma + u); });
+        if (with_beta) {
+            float2 b[P];
+            L::template load<FULL>(b, n, [&](int u) { return __ldg(beta + u); });
 #pragma unroll
-        for (int i = 0; i < UPT; ++i)
-            if (t + i * G < nunits) {
-                float g[U::N], b[U::N];
-                U::unpack(gamma[t + i * G], g);
-                if (beta) U::unpack(beta[t + i * G], b);
+            for (int e = 0; e < P; ++e) f[e] = fma2p(mul2(f[e], pk(rstd)), w[e], b[e]);
+        } else {
 #pragma unroll
-                for (int e = 0; e < U::N; ++e) {
-                    const float h = __fmul_rn(f[i][e], rstd);
-                    f[i][e] = beta ? __fmaf_rn(h, g[e], b[e]) : __fmul_rn(h, g[e]);
-                }
-                y[t + i * G] = U::pack(f[i]);
-            }
+            for (int e = 0; e < P; ++e) f[e] = mul2(mul2(f[e], pk(rstd)), w[e]);
+        }
+        L::template store<FULL>(f, n, [&](int u, const raw& out) {
+            if constexpr (UB == 16) store_vec_streaming(y + u, out);
+            else y[u] = out;
+        });
+    };
+    for (int64_t k = blockIdx.x; k < g.tiles; k += step) {
+        ok = mbar_wait_bounded(&full[s], phase) && ok;
+        // the whole warp has all its units, and all rows of the tile exist
+        if (all && (k + 1) * g.rows_per_tile <= a.rows) tile(std::true_type{}, k);
+        else tile(std::false_type{}, k);
+        if (++s == g.stages) {
+            s = 0;
+            phase ^= 1;
+        }
     }
+    if (!ok && tid == 0) atomicExch(status, 6 /* AGB_ERR_TIMEOUT */);
 }
 
 // Rows that do not fit the registers of a block: three passes over global memory.
@@ -187,8 +315,8 @@ __global__ void __launch_bounds__(1024) lna_fwd_wide(const LnaFwdArgs a) {
         }
         for (int i = threadIdx.x; i < nunits; i += G) {
             U::unpack(x[i], f);
-            U::unpack(reinterpret_cast<const raw*>(a.gamma)[i], g);
-            if (a.beta) U::unpack(reinterpret_cast<const raw*>(a.beta)[i], b);
+            U::unpack(__ldg(reinterpret_cast<const raw*>(a.gamma) + i), g);
+            if (a.beta) U::unpack(__ldg(reinterpret_cast<const raw*>(a.beta) + i), b);
 #pragma unroll
             for (int e = 0; e < U::N; ++e) {
                 const float h = __fmul_rn(__fsub_rn(f[e], mean), rstd);
@@ -218,45 +346,21 @@ struct LnaBwdArgs {
 // Rows that are no multiple of 16 bytes (UB < 16): the tile's bytes are one run all the same.  It is copied from the 16-byte boundary
 // before it to the one behind it, which lies within the tensor except at its two ends; what the ends hold beyond whole words is copied
 // by the thread itself.  Columns are then taken one by one.
-struct LnaRing {
-    int rows_per_tile, stages, tile_stride;    // bytes of a tile's slot for one array
-    int64_t tiles;
-};
-
-// Issues tile k into a slot.  `bytes` of the tensor end at `total`.
-template <bool WHOLE>
-__device__ __forceinline__ void lna_copy(uint8_t* slot, const uint8_t* base, int64_t at, int bytes, int64_t total, uint64_t* bar, int elem) {
-    if (WHOLE) {
-        bulk_load(slot, base + at, bytes, bar);
-        return;
-    }
-    const uint8_t* p = base + at;
-    const int lead = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15);
-    int lo = -lead, hi = (lead + bytes + 15) / 16 * 16 - lead;                 // relative to p
-    if (at + lo < 0) lo += 16;
-    if (at + hi > total) hi -= 16;
-    // the ends of the tensor, at most 15 bytes each (and the whole of a tile of a few bytes)
-    const int head = lo < 0 ? 0 : (lo < bytes ? lo : bytes);
-    for (int i = 0; i < head; i += elem)
-        for (int b = 0; b < elem; b += 2) *reinterpret_cast<uint16_t*>(slot + lead + i + b) = *reinterpret_cast<const uint16_t*>(p + i + b);
-    for (int i = hi > head ? hi : head; i < bytes; i += elem)
-        for (int b = 0; b < elem; b += 2) *reinterpret_cast<uint16_t*>(slot + lead + i + b) = *reinterpret_cast<const uint16_t*>(p + i + b);
-    mbar_arrive_expect_tx(bar, hi > lo ? hi - lo : 0);
-    if (hi > lo) bulk_load(slot + lead + lo, p + lo, hi - lo, bar);
-}
-
 template <typename T, int UB, int UPT, int MAXT>
 __global__ void __launch_bounds__(MAXT) lna_bwd_ring(const LnaBwdArgs a, const LnaRing g, float* partial, int* status) {
-    typedef Unit<T, UB> U;
-    typedef typename U::raw raw;
-    constexpr int N = U::N, S = 8;
+    // the slice is worked through in parts, so that the sums of all of it and the values of one part fit the registers
+    constexpr int NU = Unit<T, UB>::N, PART = UPT * NU > 8 ? (8 / NU > 0 ? 8 / NU : 1) : UPT, PARTS = UPT / PART;
+    typedef Slice<T, UB, PART> L;
+    typedef typename L::raw raw;
+    constexpr int N = L::N, P = L::P, S = 8;
     constexpr bool WHOLE = UB == 16;
     extern __shared__ __align__(128) uint8_t lna_smem[];
     __shared__ __align__(8) uint64_t full[S];
     __shared__ float2 scratch[2][32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int G = a.G, t = tid % G, mine = tid / G;            // this thread's place in its row, its row of the tile
-    const int H = a.hidden, nunits = H / N;
+    const int H = a.hidden, first = first_unit(t, G, UPT), lim = H / N - first;
+    const bool all = __all_sync(0xffffffffu, lim > 32 * (UPT - 1));
     const int64_t row_bytes = static_cast<int64_t>(H) * sizeof(T), total = a.rows * row_bytes;
     const uint8_t* xb = static_cast<const uint8_t*>(a.x);
     const uint8_t* gb = static_cast<const uint8_t*>(a.gy);
@@ -281,57 +385,57 @@ __global__ void __launch_bounds__(MAXT) lna_bwd_ring(const LnaBwdArgs a, const L
         int64_t k = blockIdx.x;
         for (int s = 0; s < g.stages && k < g.tiles; ++s, k += step) issue(k, s);
     }
-    float dg[UPT][N], db[UPT][N];
-    const raw* gamma = reinterpret_cast<const raw*>(a.gamma);   // from L1 each time: the sums take the registers
+    float2 dg[PARTS][P], db[PARTS][P];
+    const raw* gamma = reinterpret_cast<const raw*>(a.gamma) + first;   // from L1 each time: the sums take the registers
 #pragma unroll
-    for (int i = 0; i < UPT; ++i)
+    for (int i = 0; i < PARTS; ++i)
 #pragma unroll
-        for (int e = 0; e < N; ++e) dg[i][e] = db[i][e] = 0.f;
+        for (int e = 0; e < P; ++e) dg[i][e] = db[i][e] = pk(0.f);
     const float inv_h = __fdiv_rn(1.f, static_cast<float>(H));
     int s = 0, prev = 0, n = 0;
     uint32_t phase = 0;
     float next_mean = 0.f, next_rstd = 0.f;
     {
         const int64_t r = static_cast<int64_t>(blockIdx.x) * g.rows_per_tile + mine;
-        if (r < a.rows && mine < g.rows_per_tile) {
+        if (r < a.rows) {
             next_mean = a.mean[r];
             next_rstd = a.rstd[r];
         }
     }
     bool ok = true;
-    for (int64_t k = blockIdx.x; k < g.tiles; k += step, ++n) {
+    auto tile = [&](auto full_tag, int64_t k) {
+        constexpr bool FULL = decltype(full_tag)::value;
         const int64_t r = k * g.rows_per_tile + mine;
-        const bool live = r < a.rows;
         const float mean = next_mean, rstd = next_rstd;
         const int64_t rn = r + step * g.rows_per_tile;
         if (rn < a.rows) {
             next_mean = a.mean[rn];
             next_rstd = a.rstd[rn];
         }
-        ok = mbar_wait_bounded(&full[s], phase) && ok;
+        const int have = r < a.rows ? lim : 0;
         const uint8_t* slot = lna_smem + static_cast<int64_t>(2 * s) * g.tile_stride;
         const int64_t at = k * g.rows_per_tile * row_bytes;
         const int ox = WHOLE ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(xb + at) & 15);
         const int og = WHOLE ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(gb + at) & 15);
-        const raw* x = reinterpret_cast<const raw*>(slot + ox + mine * row_bytes);
-        const raw* gy = reinterpret_cast<const raw*>(slot + g.tile_stride + og + mine * row_bytes);
-        float s1 = 0.f, s2 = 0.f;
-        if (live) {
+        const raw* x = reinterpret_cast<const raw*>(slot + ox + mine * row_bytes) + first;
+        const raw* gy = reinterpret_cast<const raw*>(slot + g.tile_stride + og + mine * row_bytes) + first;
+        // columns that do not exist come as zeros of gy and gamma, which adds nothing to any of the sums
+        float2 t1 = pk(0.f), t2 = pk(0.f);
 #pragma unroll
-            for (int i = 0; i < UPT; ++i)
-                if (t + i * G < nunits) {
-                    float f[N], q[N], w[N];
-                    U::unpack(x[t + i * G], f);
-                    U::unpack(gy[t + i * G], q);
-                    U::unpack(__ldg(gamma + t + i * G), w);
+        for (int i = 0; i < PARTS; ++i) {
+            const int o = 32 * PART * i;
+            float2 f[P], q[P], w[P];
+            L::template load<FULL>(f, have - o, [&](int u) { return x[o + u]; });
+            L::template load<FULL>(q, have - o, [&](int u) { return gy[o + u]; });
+            L::template load<FULL>(w, have - o, [&](int u) { return __ldg(gamma + o + u); });
 #pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        const float v = __fmul_rn(q[e], w[e]);
-                        s1 = __fadd_rn(s1, v);
-                        s2 = __fmaf_rn(v, __fsub_rn(f[e], mean), s2);
-                    }
-                }
+            for (int e = 0; e < P; ++e) {
+                const float2 v = mul2(q[e], w[e]);
+                t1 = add2(t1, v);
+                t2 = fma2p(v, add2(f[e], pk(-mean)), t2);
+            }
         }
+        float s1 = __fadd_rn(t1.x, t1.y), s2 = __fadd_rn(t2.x, t2.y);
         for (int o = (G < 32 ? G : 32) >> 1; o > 0; o >>= 1) {
             s1 = __fadd_rn(s1, __shfl_xor_sync(0xffffffffu, s1, o));
             s2 = __fadd_rn(s2, __shfl_xor_sync(0xffffffffu, s2, o));
@@ -343,41 +447,51 @@ __global__ void __launch_bounds__(MAXT) lna_bwd_ring(const LnaBwdArgs a, const L
             if (kn < g.tiles) issue(kn, prev);
         }
         if (G > 32) {
-            const int w0 = mine * (G >> 5);
+            const int w0 = mine * (G >> 5), w1 = w0 + (G >> 5);
             s1 = s2 = 0.f;
-            for (int w = w0; w < w0 + (G >> 5); ++w) {
-                const float2 q = scratch[n & 1][w];
-                s1 = __fadd_rn(s1, q.x);
-                s2 = __fadd_rn(s2, q.y);
+            for (int w = w0; w < w1; w += 4) {         // four loads in flight
+                float2 q[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) q[u] = w + u < w1 ? scratch[n & 1][w + u] : pk(0.f);
+                s1 = __fadd_rn(s1, __fadd_rn(__fadd_rn(q[0].x, q[1].x), __fadd_rn(q[2].x, q[3].x)));
+                s2 = __fadd_rn(s2, __fadd_rn(__fadd_rn(q[0].y, q[1].y), __fadd_rn(q[2].y, q[3].y)));
             }
         }
-        if (live) {
-            const float k1 = -__fmul_rn(rstd, __fmul_rn(s1, inv_h));
-            const float k2 = -__fmul_rn(__fmul_rn(rstd, rstd), __fmul_rn(rstd, __fmul_rn(s2, inv_h)));
-            raw* dx = reinterpret_cast<raw*>(static_cast<T*>(a.dx) + r * H);
-            const raw* add = a.dx_add ? reinterpret_cast<const raw*>(static_cast<const T*>(a.dx_add) + r * H) : nullptr;
+        const float k1 = -__fmul_rn(rstd, __fmul_rn(s1, inv_h));
+        const float k2 = -__fmul_rn(__fmul_rn(rstd, rstd), __fmul_rn(rstd, __fmul_rn(s2, inv_h)));
+        raw* dx = reinterpret_cast<raw*>(static_cast<T*>(a.dx) + r * H) + first;
+        const raw* add = a.dx_add ? reinterpret_cast<const raw*>(static_cast<const T*>(a.dx_add) + r * H) + first : nullptr;
 #pragma unroll
-            for (int i = 0; i < UPT; ++i)
-                if (t + i * G < nunits) {
-                    float f[N], q[N], w[N], p[N];
-                    U::unpack(x[t + i * G], f);
-                    U::unpack(gy[t + i * G], q);
-                    U::unpack(__ldg(gamma + t + i * G), w);
-                    if (add) U::unpack(add[t + i * G], p);
+        for (int i = 0; i < PARTS; ++i) {
+            const int o = 32 * PART * i;
+            float2 f[P], q[P], w[P];
+            L::template load<FULL>(f, have - o, [&](int u) { return x[o + u]; });
+            L::template load<FULL>(q, have - o, [&](int u) { return gy[o + u]; });
+            L::template load<FULL>(w, have - o, [&](int u) { return __ldg(gamma + o + u); });
 #pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        const float xc = __fsub_rn(f[e], mean), gr = __fmul_rn(q[e], rstd);
-                        db[i][e] = __fadd_rn(db[i][e], q[e]);
-                        dg[i][e] = __fmaf_rn(gr, xc, dg[i][e]);
-                        float d = __fmaf_rn(gr, w[e], __fmaf_rn(xc, k2, k1));
-                        if (add) d = __fadd_rn(d, p[e]);
-                        f[e] = d;
-                    }
-                    const raw out = U::pack(f);
-                    if constexpr (UB == 16) store_vec_streaming(dx + t + i * G, out);
-                    else dx[t + i * G] = out;
-                }
+            for (int e = 0; e < P; ++e) {
+                const float2 xc = add2(f[e], pk(-mean)), gr = mul2(q[e], pk(rstd));
+                db[i][e] = add2(db[i][e], q[e]);
+                dg[i][e] = fma2p(gr, xc, dg[i][e]);
+                f[e] = fma2p(gr, w[e], fma2p(xc, pk(k2), pk(k1)));
+            }
+            if (add) {
+                float2 p[P];
+                L::template load<FULL>(p, have - o, [&](int u) { return add[o + u]; });
+#pragma unroll
+                for (int e = 0; e < P; ++e) f[e] = add2(f[e], p[e]);
+            }
+            L::template store<FULL>(f, have - o, [&](int u, const raw& out) {
+                if constexpr (UB == 16) store_vec_streaming(dx + o + u, out);
+                else dx[o + u] = out;
+            });
         }
+    };
+    for (int64_t k = blockIdx.x; k < g.tiles; k += step, ++n) {
+        ok = mbar_wait_bounded(&full[s], phase) && ok;
+        // the whole warp has all its units, and all rows of the tile exist
+        if (all && (k + 1) * g.rows_per_tile <= a.rows) tile(std::true_type{}, k);
+        else tile(std::false_type{}, k);
         if (g.stages == 1) {                           // a ring of one: the next tile once everyone has left this one
             __syncthreads();
             if (tid == 0 && k + step < g.tiles) issue(k + step, 0);
@@ -388,50 +502,40 @@ __global__ void __launch_bounds__(MAXT) lna_bwd_ring(const LnaBwdArgs a, const L
             phase ^= 1;
         }
     }
-    if (!ok) {
-        if (tid == 0) atomicExch(status, 6 /* AGB_ERR_TIMEOUT */);
-    }
+    if (!ok && tid == 0) atomicExch(status, 6 /* AGB_ERR_TIMEOUT */);
     if (!partial) return;
     // ---- the CTA's partial row: rows of a warp first, then warps of the same columns in order
     for (int o = 16; o >= G; o >>= 1) {
 #pragma unroll
-        for (int i = 0; i < UPT; ++i)
+        for (int i = 0; i < PARTS; ++i)
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                dg[i][e] = __fadd_rn(dg[i][e], __shfl_xor_sync(0xffffffffu, dg[i][e], o));
-                db[i][e] = __fadd_rn(db[i][e], __shfl_xor_sync(0xffffffffu, db[i][e], o));
+            for (int e = 0; e < P; ++e) {
+                dg[i][e] = add2(dg[i][e], make_float2(__shfl_xor_sync(0xffffffffu, dg[i][e].x, o), __shfl_xor_sync(0xffffffffu, dg[i][e].y, o)));
+                db[i][e] = add2(db[i][e], make_float2(__shfl_xor_sync(0xffffffffu, db[i][e].x, o), __shfl_xor_sync(0xffffffffu, db[i][e].y, o)));
             }
     }
     float* out = partial + static_cast<int64_t>(blockIdx.x) * 2 * H;
     const int per = G < 32 ? 32 : G, groups = blockDim.x / per, group = tid / per;      // threads that hold all columns once
-    if (groups == 1) {
-        if (tid < G) {
-#pragma unroll
-            for (int i = 0; i < UPT; ++i)
-                if (t + i * G < nunits)
-#pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        out[(t + i * G) * N + e] = dg[i][e];
-                        out[H + (t + i * G) * N + e] = db[i][e];
-                    }
-        }
-        return;
-    }
-    float* sums = reinterpret_cast<float*>(lna_smem);  // the ring is empty: every tile issued has been waited for
+    float* sums = groups == 1 ? out : reinterpret_cast<float*>(lna_smem);               // the ring is empty: every tile has been waited for
     for (int q = 0; q < groups; ++q) {
         __syncthreads();
-        if (group == q && tid % per < G) {
+        if (group != q || tid % per >= G) continue;
 #pragma unroll
-            for (int i = 0; i < UPT; ++i)
-                if (t + i * G < nunits)
+        for (int i = 0; i < PARTS; ++i)
 #pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        const int c = (t + i * G) * N + e;
-                        sums[c] = q ? __fadd_rn(sums[c], dg[i][e]) : dg[i][e];
-                        sums[H + c] = q ? __fadd_rn(sums[H + c], db[i][e]) : db[i][e];
-                    }
-        }
+            for (int u = 0; u < PART; ++u) {
+                const int unit = 32 * (PART * i + u);
+                if (unit >= lim) continue;
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const int c = (first + unit) * N + e;
+                    const float vg = L::at(dg[i], u * N + e), vb = L::at(db[i], u * N + e);
+                    sums[c] = q ? __fadd_rn(sums[c], vg) : vg;
+                    sums[H + c] = q ? __fadd_rn(sums[H + c], vb) : vb;
+                }
+            }
     }
+    if (groups == 1) return;
     __syncthreads();
     for (int c = tid; c < 2 * H; c += blockDim.x) out[c] = sums[c];
 }
