@@ -239,15 +239,39 @@ int check_kd(int64_t rows, int64_t vocab, int64_t k, float tau, int dtype, int i
     return AGB_OK;
 }
 
+constexpr int kKdKeep = 8;         // words of 16 bytes that a thread of a block keeps
+
 template <typename T, int MODE>
 int launch_kd(agb::KdArgs a, int64_t rows, cudaStream_t st) {
     agb_int::Device d;
     AGB_TRY(agb_int::device(&d));
-    // Slices per row: enough CTAs for the GPU where rows are few, none shorter than one turn of the block.
+    a.status = d.status;
+    const int64_t word = 16 / static_cast<int64_t>(sizeof(T));
+    const char* what = "distill_topk";
+    a.slice = a.vocab;
+    if (a.vocab <= 32 * 32 * word && a.k <= agb::kKdWarpK && rows >= d.sms) {
+        const dim3 grid(static_cast<unsigned>(ceil_div(rows, 8)));
+        if (a.vocab <= 32 * 8 * word) return launch(what, agb::kd_kernel<T, MODE, 32, 8>, grid, dim3(256), 0, st, 1, a);
+        return launch(what, agb::kd_kernel<T, MODE, 32, 0>, grid, dim3(256), 0, st, 1, a);
+    }
+    // Slices per row: enough CTAs for the GPU where rows are few, none shorter than one turn of a block of 256.
     int C = 1;
-    while (C < 8 && rows * C < 2 * d.sms && a.vocab / (2 * C) >= agb::kKdThreads * (16 / static_cast<int>(sizeof(T)))) C *= 2;
+    while (C < 8 && rows * C < 2 * d.sms && a.vocab / (2 * C) >= 256 * word) C *= 2;
+    if (MODE < 2 && C > 1 && ceil_div(a.vocab, C) <= 256 * kKdKeep * word - 64) {
+        a.slice = ceil_div(ceil_div(a.vocab, C), 64) * 64;
+        return launch(what, agb::kd_kernel<T, MODE, 256, kKdKeep>, dim3(static_cast<unsigned>(rows * C)), dim3(256), 0, st, C, a);
+    }
+    // There and back.  Long rows: blocks of 512 and slices of up to 256 KB, since a block's joins cost the same for a short one (4096 x 131072
+    // bf16: 476 us, 496 us with 256 threads and 64 KB).  Shorter rows: 256 threads (4096 x 32768 bf16: 130 us, 179 us with 512).
+    const int64_t row_bytes = a.vocab * static_cast<int64_t>(sizeof(T));
+    const bool wide = MODE == 1 && row_bytes >= (128 << 10);
+    while (wide && C < 8 && row_bytes / C > (256 << 10)) C *= 2;
     a.slice = ceil_div(ceil_div(a.vocab, C), 64) * 64;
-    return launch("distill_topk", agb::kd_kernel<T, MODE>, dim3(static_cast<unsigned>(rows * C)), dim3(agb::kKdThreads), 0, st, C, a);
+    const dim3 grid(static_cast<unsigned>(rows * C));
+    if constexpr (MODE == 1) {
+        if (wide) return launch(what, agb::kd_kernel<T, MODE, 512, 0>, grid, dim3(512), 0, st, C, a);
+    }
+    return launch(what, agb::kd_kernel<T, MODE, 256, 0>, grid, dim3(256), 0, st, C, a);
 }
 
 template <int MODE>
@@ -266,8 +290,8 @@ int run_kd(const void* z, const void* idx, int idx_type, const void* teacher, in
         AGB_TRY(check_ptr(dz, "dz", elem));
         AGB_TRY(check_ptr(dz_add, "dz_add", elem, false));
     }
-    agb::KdArgs a{z, idx, teacher, idx_type == AGB_I64, teacher_dtype == AGB_BF16, loss, lse, gy, dz_add, dz, vocab, static_cast<int>(k),
-                  tau, 1.f / tau, 0};
+    agb::KdArgs a{z, idx, teacher, idx_type == AGB_I64, teacher_dtype == AGB_BF16, loss, lse, gy, dz_add, dz, rows, vocab, static_cast<int>(k),
+                  tau, 1.f / tau, 0, nullptr};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return dtype == AGB_F32 ? launch_kd<float, MODE>(a, rows, st) : launch_kd<bf16, MODE>(a, rows, st);
 }

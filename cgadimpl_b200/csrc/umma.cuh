@@ -12,17 +12,20 @@ namespace agb {
 // hint: with the 10 us hint of mbar_try_wait the 4096 x 4096 x 18944 loss took 423 us, without it 413 us.  A poll takes 20 ns at
 // least, so the limit is 80 ms or more, against the few milliseconds of the longest tile.
 constexpr int kTcPollLimit = 1 << 22;
+__device__ __forceinline__ bool mbar_poll(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status) {
     for (int i = 0; i < kTcPollLimit; ++i) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(smem_u32(bar)), "r"(parity)
-            : "memory");
-        if (ok) return true;
+        if (mbar_poll(bar, parity)) return true;
         if (*abort_flag) return false;
     }
     *abort_flag = 1;

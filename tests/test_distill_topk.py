@@ -296,3 +296,32 @@ def test_refusals_need_no_device():
     assert bwd(one, one, 1, one, 0, one, one, odd, one, 4, 8, 2, 1.0, 0, None) == 3
     assert both(one, one, 1, one, 0, one, None, one, one, None, 4, 8, 2, 1.0, 0, None) == 1
     assert fwd(None, None, 1, None, 0, None, None, 0, 8, 2, 1.0, 0, None) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab", [(300, 9000), (310, 40003), (150, 120001), (40, 400000)])
+def test_more_rows_than_the_gpu_takes_at_once(ops, rows, vocab, dtype):
+    """Rows in turn on the same CTAs, several slices and chunks each, some without entries, against the two separate calls and the formula."""
+    z, idx, teacher, gy, add = make(rows, vocab, 7, dtype, seed=vocab, absent=0.3)
+    idx[1::5] = -1
+    z[1::5] = float("nan")
+    loss, lse = ops.distill_topk_fwd(z, idx, teacher, 2.0)
+    dz = ops.distill_topk_bwd(z, idx, teacher, lse, gy, 2.0)
+    l2, s2, d2 = ops.distill_topk_fwd_bwd(z, idx, teacher, gy, 2.0)
+    pick = torch.tensor([0, 1, 2, rows // 2, rows - 2, rows - 1], device="cuda")
+    ref = reference(z[pick], idx[pick], teacher[pick], gy[pick], 2.0)
+    tol = tolerances(z[pick], teacher[pick], gy[pick], 2.0, ref, dtype)
+    for l, s, d in ((loss, lse, dz), (l2, s2, d2)):
+        check("loss", l[pick], ref[0], tol[0])
+        check("lse", s[pick], ref[1], tol[1])
+        check("dz", d[pick], ref[2], tol[2])
+    # every row: the two ways differ by no more than both tolerances
+    assert bool(((loss - l2).abs() <= 2 * tol[0].max() * (1 + loss.abs())).all())
+    assert bool(((dz.float() - d2.float()).abs() <= 4 * half(dtype) * dz.float().abs() + 2.0 ** -14 * gy.abs()[:, None]).all())
+    assert all(torch.equal(p, q) for p, q in zip((l2, s2, d2), ops.distill_topk_fwd_bwd(z, idx, teacher, gy, 2.0)))
+    over, buf = z.clone(), add.clone()
+    assert torch.equal(ops.distill_topk_fwd_bwd(over, idx, teacher, gy, 2.0, dz=over)[2], d2)
+    got = ops.distill_topk_fwd_bwd(z, idx, teacher, gy, 2.0, dz_add=buf, dz=buf)[2]
+    ref = reference(z[pick], idx[pick], teacher[pick], gy[pick], 2.0, add[pick])
+    check("dz +=", got[pick], ref[2], tolerances(z[pick], teacher[pick], gy[pick], 2.0, ref, dtype, add[pick])[2])
