@@ -342,7 +342,8 @@ struct CePlan {
     int tn;                     // columns of a tile of logits
     int64_t pairs_per_piece;
     int splits, k_per_split;
-    size_t h, w, count, row_of, pos_of, target_of, lse_of, gy_of, gy_scale, left_over, z_target, pair_at, g, dh, dw, total;
+    int z_splits, z_per_split;  // parts of the logits' K; 1: none
+    size_t z, h, w, count, row_of, pos_of, target_of, lse_of, gy_of, gy_scale, left_over, z_target, pair_at, g, dh, dw, total;
 };
 
 // Columns of a tile of logits.  A slab of a tile takes the longest of its products (2 clocks per column), its bytes from L2 at 64 a
@@ -397,6 +398,16 @@ CePlan plan_ce(bool backward, int64_t rows, int64_t hidden, int64_t vocab, int d
     if (s < 1) s = 1;
     p.k_per_split = static_cast<int>(ceil_div(blocks, s) * agb::kTK);
     p.splits = static_cast<int>(ceil_div(p.piece, p.k_per_split));
+    // The logits of a small problem: tiles that leave most of the GPU idle, each with a long sum, are cut along it too.  1.5 us of a slab
+    // of 64 saved per eighth of the sum against one more kernel: 10 x 1835 x 2235 fp32 took 71 us as nine tiles of 174 slabs.
+    const int64_t z_tiles = ceil_div(rows, p.pair * agb::kTM) * ceil_div(vocab, agb::kTN), z_blocks = ceil_div(hidden, agb::kTK);
+    int64_t z = (sms / p.pair) / z_tiles;
+    if (z > z_blocks / 2) z = z_blocks / 2;
+    p.z_splits = 1;
+    if (p.pieces == 1 && z >= 2 && z_blocks * (p.planes == 3 ? 6 : 1) >= 40 && z * p.rows_pad * p.piece * 4 <= (64 << 20)) {
+        p.z_per_split = static_cast<int>(ceil_div(z_blocks, z) * agb::kTK);
+        p.z_splits = static_cast<int>(ceil_div(hidden, p.z_per_split));
+    }
     size_t at = 0;
     auto take = [&](size_t* where, size_t bytes) {
         *where = at;
@@ -407,6 +418,7 @@ CePlan plan_ce(bool backward, int64_t rows, int64_t hidden, int64_t vocab, int d
     take(&p.row_of, p.rows_pad * 4);
     take(&p.pos_of, p.rows_pad * 4);
     take(&p.target_of, p.rows_pad * 4);
+    if (p.z_splits > 1) take(&p.z, static_cast<size_t>(p.z_splits) * p.rows_pad * p.piece * 4);
     if (!p.direct_w) take(&p.w, static_cast<size_t>(p.planes) * p.piece * p.k_stride * 2);
     if (backward) {
         take(&p.lse_of, p.rows_pad * 4);
@@ -480,28 +492,34 @@ int ce_rows(const CeCall& c, const float* lse, const float* gy, float* loss, flo
 }
 int ce_pack(const CeCall& c, int64_t col0, int64_t n) {
     if (c.p.direct_w) return AGB_OK;
-    int64_t grid = ceil_div(n, 8);
+    const bool wide = c.hidden >= 256;
+    int64_t grid = wide ? ceil_div(n, 8) : ceil_div(n * (c.p.k_stride / 2), 256 * 8);
     if (grid > 16LL * c.d.sms) grid = 16LL * c.d.sms;
-    const dim3 g(static_cast<unsigned>(grid)), block(256);
-    const int cols = static_cast<int>(c.hidden);
+    auto pack = [&](auto kernel, auto* typed) {
+        typedef decltype(typed) P;
+        return launch("linear_ce_pack", kernel, dim3(static_cast<unsigned>(grid)), dim3(256), 0, c.st, 1, static_cast<P>(c.w) + col0 * c.hidden, n,
+                      static_cast<int>(c.hidden), c.at<bf16>(c.p.w), c.p.piece, c.p.k_stride);
+    };
     if (c.dtype == AGB_F32)
-        return launch("linear_ce_pack", agb::ce_pack_kernel<float>, g, block, 0, c.st, 1, static_cast<const float*>(c.w) + col0 * c.hidden, n, cols,
-                      c.at<bf16>(c.p.w), c.p.piece, c.p.k_stride);
-    return launch("linear_ce_pack", agb::ce_pack_kernel<bf16>, g, block, 0, c.st, 1, static_cast<const bf16*>(c.w) + col0 * c.hidden, n, cols,
-                  c.at<bf16>(c.p.w), c.p.piece, c.p.k_stride);
+        return pack(wide ? agb::ce_pack_kernel<float, true> : agb::ce_pack_kernel<float, false>, static_cast<const float*>(nullptr));
+    return pack(wide ? agb::ce_pack_kernel<bf16, true> : agb::ce_pack_kernel<bf16, false>, static_cast<const bf16*>(nullptr));
 }
 int ce_unpack(const CeCall& c, void* dw, int64_t col0, int64_t n, bool f32, int add) {
-    int64_t grid = ceil_div(n, 8);
+    const bool wide = c.hidden >= 256;
+    int64_t grid = wide ? ceil_div(n, 8) : ceil_div(n * c.hidden, 256 * 8);
     if (grid > 16LL * c.d.sms) grid = 16LL * c.d.sms;
-    const dim3 g(static_cast<unsigned>(grid)), block(256);
-    const int cols = static_cast<int>(c.hidden);
-    const char* what = "linear_ce_unpack";
+    auto unpack = [&](auto kernel, auto* from, auto* to) {
+        return launch("linear_ce_unpack", kernel, dim3(static_cast<unsigned>(grid)), dim3(256), 0, c.st, 1, from, n, static_cast<int>(c.hidden),
+                      c.p.k_stride, to + col0 * c.hidden, add);
+    };
     if (c.dtype == AGB_F32)
-        return launch(what, agb::ce_unpack_kernel<float, float>, g, block, 0, c.st, 1, c.at<float>(c.p.dw), n, cols, c.p.k_stride,
-                      static_cast<float*>(dw) + col0 * c.hidden, add);
-    bf16* to = static_cast<bf16*>(dw) + col0 * c.hidden;
-    if (f32) return launch(what, agb::ce_unpack_kernel<float, bf16>, g, block, 0, c.st, 1, c.at<float>(c.p.dw), n, cols, c.p.k_stride, to, add);
-    return launch(what, agb::ce_unpack_kernel<bf16, bf16>, g, block, 0, c.st, 1, c.at<bf16>(c.p.dw), n, cols, c.p.k_stride, to, add);
+        return unpack(wide ? agb::ce_unpack_kernel<float, float, true> : agb::ce_unpack_kernel<float, float, false>, c.at<float>(c.p.dw),
+                      static_cast<float*>(dw));
+    if (f32)
+        return unpack(wide ? agb::ce_unpack_kernel<float, bf16, true> : agb::ce_unpack_kernel<float, bf16, false>, c.at<float>(c.p.dw),
+                      static_cast<bf16*>(dw));
+    return unpack(wide ? agb::ce_unpack_kernel<bf16, bf16, true> : agb::ce_unpack_kernel<bf16, bf16, false>, c.at<bf16>(c.p.dw),
+                  static_cast<bf16*>(dw));
 }
 // W, or its piece where it was laid out: rows of the map, and the map's row of the piece's first column.
 int map_w(const CeCall& c, CUtensorMap* m, int64_t n, int box_rows) {
@@ -558,6 +576,25 @@ int launch_gemm(const CeCall& c, const agb::CeArgs& a) {
     return c.p.pair == 1 ? launch_gemm_cg<1, PHASE>(c, a) : launch_gemm_cg<2, PHASE>(c, a);
 }
 
+// The logits of a small problem as parts of K (there is one piece).
+int ce_parts(const CeCall& c) {
+    agb::CeArgs a = ce_args(c);
+    a.jobs = 1;
+    agb::CeJob& j = a.job[0];
+    j = logits_job(c, agb::kEpiDh, 0, c.vocab);
+    j.tn = agb::kTN;
+    j.b_box = j.tn / c.p.pair;
+    j.splits = c.p.z_splits;
+    j.k_per_split = c.p.z_per_split;
+    j.n_first = 1;
+    AGB_TRY(map_h(c, &a.A[0], 128));
+    AGB_TRY(map_w(c, &a.B[0], c.vocab, j.b_box));
+    a.dh = c.at<float>(c.p.z);
+    a.dh_stride = c.p.piece;
+    AGB_TRY(make_map(&a.out[0], a.dh, c.p.piece, c.p.rows_pad, c.p.z_splits, c.p.piece, c.p.rows_pad * c.p.piece, 32, true));
+    return launch_gemm<2>(c, a);
+}
+
 int start_ce(CeCall* c, bool backward, bool want_dh, void* workspace, size_t workspace_bytes, agb_stream_t stream) {
     const int elem = c->dtype == AGB_F32 ? 4 : 2;
     AGB_TRY(check_ptr(c->h, "h", elem));
@@ -594,6 +631,18 @@ int agb_linear_ce_fwd(const void* h, const void* w, const void* target, int targ
     CeCall c{h, w, target, target_type, rows, hidden, vocab, dtype, nullptr, nullptr, {}, {}};
     AGB_TRY(start_ce(&c, false, false, workspace, workspace_bytes, stream));
     AGB_TRY(ce_rows(c, nullptr, nullptr, loss, lse));
+    if (c.p.z_splits > 1) {
+        AGB_TRY(ce_pack(c, 0, vocab));
+        AGB_TRY(ce_parts(c));
+        auto join = [&](auto kernel, auto* typed) {
+            typedef decltype(typed) P;
+            return launch("linear_ce_join_parts", kernel, dim3(static_cast<unsigned>(rows)), dim3(256), 0, c.st, 1, c.at<float>(c.p.z), c.p.z_splits,
+                          c.p.rows_pad, c.p.piece, static_cast<int>(vocab), c.at<int>(c.p.count), c.at<int>(c.p.target_of), c.at<int>(c.p.row_of),
+                          static_cast<P>(h), static_cast<P>(w), static_cast<int>(hidden), loss, lse);
+        };
+        return dtype == AGB_F32 ? join(agb::ce_join_parts_kernel<float>, static_cast<const float*>(nullptr))
+                                : join(agb::ce_join_parts_kernel<bf16>, static_cast<const bf16*>(nullptr));
+    }
     for (int64_t i = 0; i < c.p.pieces; ++i) {
         const int64_t col0 = i * c.p.piece, n = vocab - col0 < c.p.piece ? vocab - col0 : c.p.piece;
         AGB_TRY(ce_pack(c, col0, n));
@@ -659,7 +708,15 @@ int agb_linear_ce_bwd(const void* h, const void* w, const void* target, int targ
         a.left_over = c.p.planes == 1 ? c.at<float>(c.p.left_over) : nullptr;
         a.gy_scale = c.at<float>(c.p.gy_scale);
         AGB_TRY(map_g(c, &a.out[0], 32));
-        AGB_TRY(c.p.planes == 1 ? launch_gemm<1>(c, a) : launch_gemm<3>(c, a));
+        if (c.p.z_splits > 1) {
+            AGB_TRY(ce_parts(c));
+            const dim3 grid(static_cast<unsigned>(ceil_div(c.p.g_stride, 512)), static_cast<unsigned>(ceil_div(rows, agb::kTK) * agb::kTK));
+            AGB_TRY(launch("linear_ce_g_parts", agb::ce_g_parts_kernel, grid, dim3(256), 0, c.st, 1, c.at<float>(c.p.z), c.p.z_splits, c.p.rows_pad,
+                           c.p.piece, static_cast<int>(vocab), c.at<int>(c.p.count), c.at<int>(c.p.target_of), a.lse, a.gy, a.gy_scale, a.g,
+                           a.g_stride, c.p.planes, a.left_over));
+        } else {
+            AGB_TRY(c.p.planes == 1 ? launch_gemm<1>(c, a) : launch_gemm<3>(c, a));
+        }
         a.jobs = 0;
         if (dh) {
             agb::CeJob& j = a.job[a.jobs];

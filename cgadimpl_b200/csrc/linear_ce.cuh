@@ -298,14 +298,49 @@ __global__ void __launch_bounds__(256) ce_rows_kernel(const CeRowsArgs a) {
             ce_copy_row(static_cast<const T*>(a.x) + (r0 + i) * a.cols, a.dst + where[i] * a.stride, a.cols, a.stride, plane, vec, lane);
 }
 
-// Rows [row0, row0 + rows) of w into dst [planes][rows_pad][stride]: what W needs where TMA cannot read it as it is.
-template <typename T>
+// Rows [row0, row0 + rows) of w into dst [planes][rows_pad][stride]: what W needs where TMA cannot read it as it is.  LONG: a warp per row.
+// Else a thread takes pairs of columns wherever they lie, so that short rows fill the warps too, at the price of a division per pair.
+template <typename T, bool LONG>
 __global__ void __launch_bounds__(256) ce_pack_kernel(const T* w, int64_t rows, int cols, __nv_bfloat16* dst, int64_t rows_pad, int64_t stride) {
     pdl_wait();
     pdl_trigger();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + warp; r < rows; r += static_cast<int64_t>(gridDim.x) * 8)
-        ce_copy_row(w + r * cols, dst + r * stride, cols, stride, rows_pad * stride, false, lane);
+    if constexpr (LONG) {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        for (int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + warp; r < rows; r += static_cast<int64_t>(gridDim.x) * 8)
+            ce_copy_row(w + r * cols, dst + r * stride, cols, stride, rows_pad * stride, false, lane);
+        return;
+    }
+    constexpr int B = 8;
+    const uint32_t per_row = static_cast<uint32_t>(stride / 2);
+    const int64_t total = rows * per_row, step = static_cast<int64_t>(gridDim.x) * 256, p32 = rows_pad * per_row;
+    uint32_t* d = reinterpret_cast<uint32_t*>(dst);
+    for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i0 < total; i0 += step * B) {
+        T v[B][2];
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const int64_t i = i0 + b * step;
+            const uint32_t r = static_cast<uint32_t>(i < total ? i : 0) / per_row;      // a piece has less than 2^32 pairs
+            const int c = 2 * static_cast<int>(static_cast<uint32_t>(i < total ? i : 0) - r * per_row);
+            const T* src = w + static_cast<int64_t>(r) * cols + c;
+            v[b][0] = i < total && c < cols ? src[0] : T(0.f);
+            v[b][1] = i < total && c + 1 < cols ? src[1] : T(0.f);
+        }
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const int64_t i = i0 + b * step;
+            if (i >= total) continue;
+            if (sizeof(T) == 2) {
+                d[i] = (__float_as_uint(Vec<T>::load1(&v[b][0])) >> 16) | (__float_as_uint(Vec<T>::load1(&v[b][1])) & 0xffff0000u);
+            } else {
+                uint32_t h0, m0, l0, h1, m1, l1;
+                split3(Vec<T>::load1(&v[b][0]), h0, m0, l0);
+                split3(Vec<T>::load1(&v[b][1]), h1, m1, l1);
+                d[i] = (h0 >> 16) | h1;
+                d[p32 + i] = (m0 >> 16) | m1;
+                d[2 * p32 + i] = (l0 >> 16) | l1;
+            }
+        }
+    }
 }
 
 // ---------------------------------------------------------------- the epilogue's stores
@@ -326,13 +361,30 @@ __device__ __forceinline__ void ce_send(uint8_t* boxes, int& turn, const uint4 (
     }
 }
 
-// A staged piece of dw [rows][stride] (S: bf16, or fp32 that is still to be rounded or added) to its place [rows][cols].  A warp per row;
-// 16-bit rows that start between two words are written as a single element and pairs.
-template <typename S, typename T>
+// A staged piece of dw [rows][stride] (S: bf16, or fp32 that is still to be rounded or added) to its place [rows][cols].  LONG: a warp per row;
+// 16-bit rows that start between two words are written as a single element and pairs.  Else element by element, wherever they lie.
+template <typename S, typename T, bool LONG>
 __global__ void __launch_bounds__(256) ce_unpack_kernel(const S* src, int64_t rows, int cols, int64_t stride, T* dw, int add) {
     constexpr int B = 8;
     pdl_wait();
     pdl_trigger();
+    if constexpr (!LONG) {
+        const int64_t total = rows * cols, step = static_cast<int64_t>(gridDim.x) * 256;
+        for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i0 < total; i0 += step * B) {
+            float v[B], o[B];
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const int64_t i = i0 + b * step;
+                const uint32_t at = static_cast<uint32_t>(i < total ? i : 0), r = at / cols;   // a piece has less than 2^32 elements
+                v[b] = Vec<S>::load1(src + static_cast<int64_t>(r) * stride + (at - r * cols));
+                o[b] = add ? Vec<T>::load1(dw + at) : 0.f;
+            }
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+                if (i0 + b * step < total) Vec<T>::store1(dw + i0 + b * step, add ? __fadd_rn(v[b], o[b]) : v[b]);
+        }
+        return;
+    }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + warp; r < rows; r += static_cast<int64_t>(gridDim.x) * 8) {
         const S* s = src + r * stride;
@@ -740,6 +792,105 @@ __global__ void __launch_bounds__(256) ce_join_kernel(const float2* pairs, int n
     const float l = __fadd_rn(m, logf(s));
     lse[r] = l;
     loss[r] = __fsub_rn(l, z);
+}
+
+// Few tiles and a long sum: the logits as fp32 parts [splits][rows_pad][stride] of K, each part a CTA's.  This is the join for them: a block
+// per row adds the parts, takes the maximum and the sum, and goes on as ce_join_kernel does.
+template <typename T>
+__global__ void __launch_bounds__(256) ce_join_parts_kernel(const float* parts, int splits, int64_t rows_pad, int64_t stride, int vocab,
+                                                            const int* count, const int* target_of, const int* row_of, const T* h, const T* w,
+                                                            int hidden, float* loss, float* lse) {
+    __shared__ float red[8][3];
+    __shared__ float z_there;
+    pdl_wait();
+    pdl_trigger();
+    const int i = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (i >= *count) return;
+    const int r = row_of[i], target = target_of[i];
+    float z = 0.f;
+    const T* hr = h + static_cast<int64_t>(r) * hidden;
+    const T* wr = w + static_cast<int64_t>(target) * hidden;
+#pragma unroll 4
+    for (int c = threadIdx.x; c < hidden; c += 256) z = __fmaf_rn(Vec<T>::load1(hr + c), Vec<T>::load1(wr + c), z);
+    float m = -INFINITY, s = 0.f;
+    const float* p = parts + i * stride;
+#pragma unroll 2
+    for (int c = threadIdx.x * 4; c < vocab; c += 1024) {
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int k = 0; k < splits; ++k) {
+            const float4 q = *reinterpret_cast<const float4*>(p + k * rows_pad * stride + c);
+            v[0] = __fadd_rn(v[0], q.x);
+            v[1] = __fadd_rn(v[1], q.y);
+            v[2] = __fadd_rn(v[2], q.z);
+            v[3] = __fadd_rn(v[3], q.w);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (c + e == target) z_there = v[e];
+            if (c + e >= vocab) v[e] = -INFINITY;
+        }
+        online_add(v, 1.f, m, s);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        z = __fadd_rn(z, __shfl_xor_sync(0xffffffffu, z, o));
+        const float mb = __shfl_xor_sync(0xffffffffu, m, o), sb = __shfl_xor_sync(0xffffffffu, s, o);
+        join_pair(m, s, mb, sb);
+    }
+    if (lane == 0) {
+        red[warp][0] = z;
+        red[warp][1] = m;
+        red[warp][2] = s;
+    }
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int q = 1; q < 8; ++q) {
+        z = __fadd_rn(z, red[q][0]);
+        join_pair(m, s, red[q][1], red[q][2]);
+    }
+    s = __fadd_rn(s, __fsub_rn(exp2f(__fmul_rn(__fsub_rn(z, m), kLog2e)), exp2f(__fmul_rn(__fsub_rn(z_there, m), kLog2e))));
+    const float l = __fadd_rn(m, logf(s));
+    lse[r] = l;
+    loss[r] = __fsub_rn(l, z);
+}
+
+// g of the same parts, what the epilogue of PHASE 1 (3) writes; zeros up to whole slabs of rows and columns.
+__global__ void __launch_bounds__(256) ce_g_parts_kernel(const float* parts, int splits, int64_t rows_pad, int64_t stride, int vocab,
+                                                         const int* count, const int* target_of, const float* lse_of, const float* gy_of,
+                                                         const float* gy_scale, __nv_bfloat16* g, int64_t g_stride, int planes, float* left_over) {
+    pdl_wait();
+    pdl_trigger();
+    const int i = blockIdx.y, c = (blockIdx.x * 256 + threadIdx.x) * 2, n = *count;
+    if (i >= (n + kTK - 1) / kTK * kTK || c >= g_stride) return;
+    float v[2] = {0.f, 0.f};
+    if (i < n) {
+        const float lse = lse_of[i], gy = __fdiv_rn(gy_of[i], *gy_scale);
+        const int target = target_of[i];
+        const float* p = parts + i * stride + c;
+        float2 z = make_float2(0.f, 0.f);
+#pragma unroll 4
+        for (int k = 0; k < splits; ++k) z = add2(z, *reinterpret_cast<const float2*>(p + k * rows_pad * stride));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float q = ex2f(__fmul_rn(__fsub_rn(e ? z.y : z.x, lse), kLog2e));
+            if (target == c + e) q = __fsub_rn(q, 1.f);
+            v[e] = c + e < vocab ? __fmul_rn(gy, q) : 0.f;
+            if (planes == 1 && target == c + e) left_over[i] = __fsub_rn(v[e], __bfloat162float(__float2bfloat16_rn(v[e])));
+        }
+    }
+    uint32_t* o = reinterpret_cast<uint32_t*>(g + i * g_stride + c);
+    if (planes == 1) {
+        *o = pack_bf16x2(v[0], v[1]);
+    } else {
+        const int64_t plane = rows_pad * g_stride / 2;
+        uint32_t h0, m0, l0, h1, m1, l1;
+        split3(v[0], h0, m0, l0);
+        split3(v[1], h1, m1, l1);
+        o[0] = (h0 >> 16) | h1;
+        o[plane] = (m0 >> 16) | m1;
+        o[2 * plane] = (l0 >> 16) | l1;
+    }
 }
 
 // dh of every row: the parts summed in order, what rounding took from g at the target times that row of W, rounded once; zeros where

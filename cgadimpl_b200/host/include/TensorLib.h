@@ -17,10 +17,11 @@
 
 namespace OwnTensor {
 
-enum class Dtype : uint8_t { Float32 = 0, Bfloat16 = 1, Float64 = 2 };
+// Int32 and Int64 hold indices (targets, teacher columns); no rule differentiates them.
+enum class Dtype : uint8_t { Float32 = 0, Bfloat16 = 1, Float64 = 2, Int32 = 3, Int64 = 4 };
 enum class Device : uint8_t { CPU = 0, CUDA = 1 };
 
-inline size_t dtype_size(Dtype d) { return d == Dtype::Float32 ? 4 : (d == Dtype::Bfloat16 ? 2 : 8); }
+inline size_t dtype_size(Dtype d) { return d == Dtype::Float32 || d == Dtype::Int32 ? 4 : (d == Dtype::Bfloat16 ? 2 : 8); }
 
 struct DeviceIndex {
     Device device{Device::CPU};
@@ -104,6 +105,7 @@ public:
     static Tensor randn(const Shape& s, const TensorOptions& o = {});
     static Tensor rand(const Shape& s, const TensorOptions& o = {});
     static Tensor from_host(const float* data, const Shape& s, const TensorOptions& o = {});
+    static Tensor from_host(const int64_t* data, const Shape& s, const TensorOptions& o);   // Int32 or Int64
 
     const Shape& shape() const { return shape_; }
     int64_t numel() const { return numel_; }

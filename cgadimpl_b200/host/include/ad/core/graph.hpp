@@ -61,7 +61,7 @@ struct Node : std::enable_shared_from_this<Node> {
     };
     ExecutionContext creation_context;
 
-    float eps{1e-5f};  // normalisation nodes only (the reference hard-codes 1e-5)
+    float eps{1e-5f};  // normalisation nodes (the reference hard-codes 1e-5); the temperature of a distillation loss
 
     bool requires_grad_flag_{false};
     bool requires_grad() const { return requires_grad_flag_; }

@@ -21,6 +21,14 @@ inline int agb_dtype(const Tensor& t) {
     }
 }
 
+inline int agb_index(const Tensor& t, const char* what) {
+    switch (t.dtype()) {
+        case Dtype::Int32: return AGB_I32;
+        case Dtype::Int64: return AGB_I64;
+        default: throw std::runtime_error(std::string(what) + ": an Int32 or Int64 tensor is needed");
+    }
+}
+
 inline void require_cuda(const Tensor& t, const char* what) {
     if (!t.is_cuda())
         throw std::runtime_error(std::string(what) + ": tensor is on the CPU; this path has no CPU implementation");

@@ -30,5 +30,10 @@ std::shared_ptr<Node> rmsnorm_nodeops(const std::shared_ptr<Node>& x, const std:
 std::shared_ptr<Node> add_rmsnorm_nodeops(const std::shared_ptr<Node>& x, const std::shared_ptr<Node>& r,
                                           const std::shared_ptr<Node>& gamma, float eps);
 
+std::shared_ptr<Node> layernorm_nodeops(const std::shared_ptr<Node>& x, const std::shared_ptr<Node>& gamma,
+                                        const std::shared_ptr<Node>& beta, float eps);   // beta may be null
+std::shared_ptr<Node> linear_cross_entropy_nodeops(const std::shared_ptr<Node>& h, const std::shared_ptr<Node>& w, const Tensor& target);
+std::shared_ptr<Node> distill_topk_nodeops(const std::shared_ptr<Node>& z, const Tensor& idx, const Tensor& teacher, float temperature);
+
 }  // namespace detail
 }  // namespace ag

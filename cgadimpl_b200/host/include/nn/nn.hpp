@@ -42,6 +42,20 @@ private:
     float eps_;
 };
 
+// LayerNorm with weight and bias: gamma and beta [hidden], ones and zeros.
+class LayerNorm : public Module {
+public:
+    LayerNorm(int64_t hidden, float eps = 1e-5f, bool bias = true, DeviceIndex dev = DeviceIndex(Device::CUDA), Dtype dtype = Dtype::Float32);
+    using Module::operator();
+    Value operator()(Value input) override;
+    Value& gamma() { return params_[0]; }
+    Value& beta() { return params_.at(1); }             // throws without a bias
+    float eps() const { return eps_; }
+
+private:
+    float eps_;
+};
+
 class Sequential : public Module {
 public:
     explicit Sequential(const std::vector<Module*>& modules);

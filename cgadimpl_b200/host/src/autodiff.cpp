@@ -63,11 +63,11 @@ void run_hooks(Node* n) {
 // mean, var) and softmax its own value.
 bool rule_reads_inputs(Op op) {
     return op == Op::Mul || op == Op::RMSNorm || op == Op::RMSNormAffine || op == Op::RealRMSNorm || op == Op::LayerNorm ||
-           op == Op::LogSumExpRow;
+           op == Op::LogSumExpRow || op == Op::CeWithLogits || op == Op::KLDivergence;
 }
 bool rule_reads_own_tape(Op op) {
     return op == Op::RMSNorm || op == Op::RMSNormAffine || op == Op::RealRMSNorm || op == Op::LayerNorm ||
-           op == Op::SoftmaxRow;
+           op == Op::SoftmaxRow || op == Op::CeWithLogits || op == Op::KLDivergence;
 }
 
 // Runs n's rule with every activation it reads present: dropped ones are recomputed first

@@ -31,6 +31,16 @@ RMSNorm::RMSNorm(int64_t hidden, float eps, DeviceIndex dev, Dtype dtype) : eps_
 Value RMSNorm::operator()(Value input) { return ag::rmsnorm(input, params_[0], eps_); }
 Value RMSNorm::operator()(Value x, Value residual) { return ag::add_rmsnorm(x, residual, params_[0], eps_); }
 
+LayerNorm::LayerNorm(int64_t hidden, float eps, bool bias, DeviceIndex dev, Dtype dtype) : eps_(eps) {
+    if (hidden < 1) throw std::invalid_argument("LayerNorm: hidden must be positive");
+    const auto o = TensorOptions().with_device(dev).with_dtype(dtype).with_req_grad(true);
+    params_.push_back(make_tensor(Tensor::ones(Shape{{hidden}}, o), "gamma"));
+    if (bias) params_.push_back(make_tensor(Tensor::zeros(Shape{{hidden}}, o), "beta"));
+}
+Value LayerNorm::operator()(Value input) {
+    return params_.size() > 1 ? ag::layernorm(input, params_[0], params_[1], eps_) : ag::layernorm(input, params_[0], eps_);
+}
+
 Sequential::Sequential(const std::vector<Module*>& modules) : layers_(modules) {
     for (auto* m : layers_)
         for (auto& p : m->parameters()) params_.push_back(p);

@@ -329,6 +329,112 @@ std::shared_ptr<Node> logsumexp_row_nodeops(const std::shared_ptr<Node>& z) {
     return n;
 }
 
+namespace {
+Shape row_shape(const Tensor& t) {
+    Shape s = t.shape();
+    if (s.dims.empty()) s.dims.push_back(1);
+    s.dims.back() = 1;
+    return s;
+}
+void same_place(const Tensor& a, const Tensor& b, const char* what) {
+    require_cuda(a, what);
+    require_cuda(b, what);
+    if (a.device() != b.device()) throw std::runtime_error(std::string(what) + ": operands live on different devices");
+}
+struct LayerNormAffineOut {
+    Tensor y, mean, rstd;
+};
+LayerNormAffineOut layernorm_affine_forward(const Tensor& x, const Tensor& gamma, const Tensor* beta, float eps) {
+    const auto rh = rows_hidden(x);
+    for (const Tensor* p : {&gamma, beta}) {
+        if (!p) continue;
+        same_place(x, *p, "layernorm");
+        if (p->numel() != rh.hidden || p->shape().dims.back() != rh.hidden)
+            throw std::runtime_error("layernorm: gamma and beta must have shape [hidden] (or [1, hidden])");
+        if (p->dtype() != x.dtype()) throw std::runtime_error("layernorm: gamma, beta and x must have the same dtype");
+    }
+    StreamGuard g(current_stream());
+    LayerNormAffineOut o;
+    const auto f32 = TensorOptions().with_dtype(Dtype::Float32).with_device(x.device());
+    o.y = Tensor(x.shape(), ag::options(x).with_req_grad(false));
+    o.mean = Tensor(row_shape(x), f32);
+    o.rstd = Tensor(row_shape(x), f32);
+    check_status(agb_layernorm_affine_fwd(x.raw(), gamma.raw(), beta ? beta->raw() : nullptr, o.y.raw(), o.mean.data<float>(),
+                                          o.rstd.data<float>(), rh.rows, rh.hidden, eps, agb_dtype(x), current_stream()),
+                 "layernorm forward");
+    return o;
+}
+struct RowLossOut {
+    Tensor loss, lse;
+};
+RowLossOut linear_ce_forward(const Tensor& h, const Tensor& w, const Tensor& target) {
+    same_place(h, w, "linear_cross_entropy");
+    same_place(h, target, "linear_cross_entropy");
+    const auto rh = rows_hidden(h);
+    const auto& wd = w.shape().dims;
+    if (wd.size() != 2 || wd[1] != rh.hidden || w.dtype() != h.dtype())
+        throw std::runtime_error("linear_cross_entropy: w must be [vocab, hidden] with h's dtype");
+    if (target.numel() != rh.rows) throw std::runtime_error("linear_cross_entropy: one target per row of h");
+    StreamGuard g(current_stream());
+    const auto f32 = TensorOptions().with_dtype(Dtype::Float32).with_device(h.device());
+    RowLossOut o{Tensor(row_shape(h), f32), Tensor(row_shape(h), f32)};
+    const size_t wsb = agb_linear_ce_workspace_bytes(0, rh.rows, rh.hidden, wd[0], agb_dtype(h));
+    check_status(agb_linear_ce_fwd(h.raw(), w.raw(), target.raw(), agb_index(target, "linear_cross_entropy"), o.loss.data<float>(),
+                                   o.lse.data<float>(), rh.rows, rh.hidden, wd[0], agb_dtype(h), workspace(wsb, h, current_stream()), wsb,
+                                   current_stream()),
+                 "linear_cross_entropy forward");
+    return o;
+}
+RowLossOut distill_forward(const Tensor& z, const Tensor& idx, const Tensor& teacher, float temperature) {
+    same_place(z, idx, "distill_topk");
+    same_place(z, teacher, "distill_topk");
+    const auto rh = rows_hidden(z);
+    if (idx.shape().dims != teacher.shape().dims || rh.rows == 0 || idx.numel() % rh.rows || idx.numel() == 0)
+        throw std::runtime_error("distill_topk: idx and teacher must both be [rows.., k]");
+    StreamGuard g(current_stream());
+    const auto f32 = TensorOptions().with_dtype(Dtype::Float32).with_device(z.device());
+    RowLossOut o{Tensor(row_shape(z), f32), Tensor(row_shape(z), f32)};
+    check_status(agb_distill_topk_fwd(z.raw(), idx.raw(), agb_index(idx, "distill_topk"), teacher.raw(), agb_dtype(teacher), o.loss.data<float>(),
+                                      o.lse.data<float>(), rh.rows, rh.hidden, idx.numel() / rh.rows, temperature, agb_dtype(z),
+                                      current_stream()),
+                 "distill_topk forward");
+    return o;
+}
+}  // namespace
+
+// inputs = {x, gamma[, beta]}; tape = {mean, rstd}, both [.., 1] fp32.
+std::shared_ptr<Node> layernorm_nodeops(const std::shared_ptr<Node>& x, const std::shared_ptr<Node>& gamma, const std::shared_ptr<Node>& beta,
+                                        float eps) {
+    LayerNormAffineOut o = layernorm_affine_forward(x->value, gamma->value, beta ? &beta->value : nullptr, eps);
+    auto n = std::make_shared<Node>(o.y, Op::LayerNorm, x->requires_grad() || gamma->requires_grad() || (beta && beta->requires_grad()),
+                                    "layernorm");
+    n->eps = eps;
+    n->tape.push_back(std::make_shared<Tensor>(o.mean));
+    n->tape.push_back(std::make_shared<Tensor>(o.rstd));
+    if (beta) link(n, {x, gamma, beta});
+    else link(n, {x, gamma});
+    return n;
+}
+
+// inputs = {h, w, target}; the target is a leaf without a gradient; tape = {lse}.
+std::shared_ptr<Node> linear_cross_entropy_nodeops(const std::shared_ptr<Node>& h, const std::shared_ptr<Node>& w, const Tensor& target) {
+    RowLossOut o = linear_ce_forward(h->value, w->value, target);
+    auto n = std::make_shared<Node>(o.loss, Op::CeWithLogits, h->requires_grad() || w->requires_grad(), "linear_cross_entropy");
+    n->tape.push_back(std::make_shared<Tensor>(o.lse));
+    link(n, {h, w, std::make_shared<Node>(target, Op::Leaf, false, "target")});
+    return n;
+}
+
+// inputs = {z, idx, teacher}, the last two leaves without gradients; eps holds the temperature; tape = {lse}.
+std::shared_ptr<Node> distill_topk_nodeops(const std::shared_ptr<Node>& z, const Tensor& idx, const Tensor& teacher, float temperature) {
+    RowLossOut o = distill_forward(z->value, idx, teacher, temperature);
+    auto n = std::make_shared<Node>(o.loss, Op::KLDivergence, z->requires_grad(), "distill_topk");
+    n->eps = temperature;
+    n->tape.push_back(std::make_shared<Tensor>(o.lse));
+    link(n, {z, std::make_shared<Node>(idx, Op::Leaf, false, "teacher_columns"), std::make_shared<Node>(teacher, Op::Leaf, false, "teacher")});
+    return n;
+}
+
 }  // namespace detail
 
 // Recomputes a node's value from its inputs' values -- and its tape, which the rules of the norm
@@ -372,9 +478,24 @@ Tensor forward_eval_node(Node* node) {
             return o.y;
         }
         case Op::LayerNorm: {
+            if (node->inputs.size() > 1) {
+                LayerNormAffineOut o = layernorm_affine_forward(in(0), in(1), node->inputs.size() > 2 ? &in(2) : nullptr, node->eps);
+                set_tape({o.mean, o.rstd});
+                return o.y;
+            }
             LayerNormOut o = layernorm_forward(in(0), node->eps);
             set_tape({o.var, o.mean});
             return o.y;
+        }
+        case Op::CeWithLogits: {
+            RowLossOut o = linear_ce_forward(in(0), in(1), in(2));
+            set_tape({o.lse});
+            return o.loss;
+        }
+        case Op::KLDivergence: {
+            RowLossOut o = distill_forward(in(0), in(1), in(2), node->eps);
+            set_tape({o.lse});
+            return o.loss;
         }
         case Op::SoftmaxRow: return softmax_family_forward(in(0), false);
         case Op::LogSumExpRow: return softmax_family_forward(in(0), true);
@@ -402,6 +523,16 @@ Value logsumexp_row(const Value& z) { return Value(detail::logsumexp_row_nodeops
 Value rmsnorm(const Value& x, const Value& gamma, float eps) { return Value(detail::rmsnorm_nodeops(x.node, gamma.node, eps)); }
 Value add_rmsnorm(const Value& x, const Value& r, const Value& gamma, float eps) {
     return Value(detail::add_rmsnorm_nodeops(x.node, r.node, gamma.node, eps));
+}
+Value layernorm(const Value& x, const Value& gamma, const Value& beta, float eps) {
+    return Value(detail::layernorm_nodeops(x.node, gamma.node, beta.node, eps));
+}
+Value layernorm(const Value& x, const Value& gamma, float eps) { return Value(detail::layernorm_nodeops(x.node, gamma.node, nullptr, eps)); }
+Value linear_cross_entropy(const Value& h, const Value& w, const Tensor& target) {
+    return Value(detail::linear_cross_entropy_nodeops(h.node, w.node, target));
+}
+Value distill_topk(const Value& z, const Tensor& idx, const Tensor& teacher, float temperature) {
+    return Value(detail::distill_topk_nodeops(z.node, idx, teacher, temperature));
 }
 Value residual_of(const Value& y) {
     if (!y.node || y.node->op != Op::RMSNormAffine || y.node->inputs.empty() || y.node->inputs[0]->op != Op::Add)

@@ -71,6 +71,21 @@ Tensor jvp_LayerNorm(Node* n, const TangentOf& t) {
     require_cuda(n->value, "laynor jvp");
     StreamGuard g(current_stream());
     const auto rh = rows_hidden(n->value);
+    if (n->inputs.size() > 1) {                        // ty = t(xh) * gamma + xh * t(gamma) [+ t(beta)], xh formed again
+        const Tensor &x = n->inputs[0]->value, &gamma = n->inputs[1]->value;
+        const auto f32 = TensorOptions().with_dtype(Dtype::Float32).with_device(x.device());
+        Tensor xh(x.shape(), ag::options(x).with_req_grad(false)), th(x.shape(), ag::options(x).with_req_grad(false));
+        Tensor mean(n->tape[0]->shape(), f32), var(n->tape[0]->shape(), f32);
+        check_status(agb_layernorm_fwd(x.raw(), xh.raw(), mean.data<float>(), var.data<float>(), rh.rows, rh.hidden, n->eps, agb_dtype(x),
+                                       current_stream()),
+                     "layernorm jvp");
+        check_status(agb_layernorm_jvp(xh.raw(), tx.raw(), var.data<float>(), th.raw(), rh.rows, rh.hidden, n->eps, agb_dtype(x),
+                                       current_stream()),
+                     "layernorm jvp");
+        Tensor out = binary_op(0, binary_op(1, th, gamma, current_stream()),
+                               binary_op(1, xh, tangent(t, n->inputs[1].get()), current_stream()), current_stream());
+        return n->inputs.size() > 2 ? binary_op(0, out, tangent(t, n->inputs[2].get()), current_stream()) : out;
+    }
     Tensor out(n->value.shape(), ag::options(n->value).with_req_grad(false));
     check_status(agb_layernorm_jvp(n->value.raw(), tx.raw(), n->tape[0]->data<float>(), out.raw(), rh.rows, rh.hidden, n->eps,
                                    agb_dtype(n->value), current_stream()),

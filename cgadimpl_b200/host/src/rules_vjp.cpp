@@ -3,6 +3,9 @@
 // Every rule launches on the node's creation stream (the reference's current_stream() is
 // thread-local and therefore null in the worker threads of the parallel backward).
 #define AG_EXPOSE_AUTODIFF_RULES
+#include <algorithm>
+#include <vector>
+
 #include "ad/detail/autodiff_ops.hpp"
 #include "ad/detail/host_util.hpp"
 
@@ -73,6 +76,55 @@ void norm_backward(Node* X, Node* G, const Tensor& rstd, const Tensor& gy, ag_cu
                  "rmsnorm backward");
 }
 
+// The locks of several parents in one order (two rules that share parents run at once in the parallel backward), a parent named
+// twice locked once.
+struct GradLocks {
+    std::vector<std::unique_lock<std::mutex>> held;
+    explicit GradLocks(std::vector<Node*> nodes) {
+        std::sort(nodes.begin(), nodes.end());
+        nodes.erase(std::unique(nodes.begin(), nodes.end()), nodes.end());
+        for (Node* p : nodes)
+            if (p) held.emplace_back(p->grad_mutex);
+    }
+};
+
+// LayerNorm with weight and bias: dx is added in place (dx_add == dx), the column sums accumulate in fp32.
+void layernorm_affine_backward(Node* n, const Tensor& gy, ag_cuda_stream_t st) {
+    Node* X = n->inputs[0].get();
+    Node* G = n->inputs[1].get();
+    Node* B = n->inputs.size() > 2 ? n->inputs[2].get() : nullptr;
+    const Tensor& x = X->value;
+    const auto rh = rows_hidden(x);
+    const bool want_dx = X->requires_grad(), want_dg = G->requires_grad(), want_db = B && B->requires_grad();
+    if (!want_dx && !want_dg && !want_db) return;
+    for (Node* p : {want_dg ? G : nullptr, want_db ? B : nullptr})
+        if (p && p->value.dtype() != Dtype::Float32)
+            throw std::runtime_error("layernorm backward: the gradients of gamma and beta are produced in fp32; a non-fp32 node cannot receive "
+                                     "them through the graph API (use agb_layernorm_affine_bwd directly)");
+    if ((want_dg && (G == X || G == B)) || (want_db && B == X))
+        throw std::runtime_error("layernorm backward: x, gamma and beta must be different nodes");
+    const size_t wsb = want_dg || want_db ? agb_layernorm_affine_bwd_workspace_bytes(rh.rows, rh.hidden, agb_dtype(x)) : 0;
+    void* ws = wsb ? workspace(wsb, x, st) : nullptr;
+    Tensor scratch;
+    if (!want_dx) scratch = Tensor(x.shape(), ag::options(x).with_req_grad(false));
+    GradLocks locks({want_dx ? X : nullptr, want_dg ? G : nullptr, want_db ? B : nullptr});
+    bool first_dx = false, first_dg = false, first_db = false;
+    Tensor* gx = want_dx ? &X->open_grad(&first_dx) : nullptr;
+    Tensor* gg = want_dg ? &G->open_grad(&first_dg) : nullptr;
+    Tensor* gb = want_db ? &B->open_grad(&first_db) : nullptr;
+    if (gg && gb && first_dg != first_db) {            // one of the two has a contribution already: both add
+        if (first_dg) gg->zero_();
+        else gb->zero_();
+        first_dg = first_db = false;
+    }
+    const bool add_columns = gg ? !first_dg : !first_db;
+    check_status(agb_layernorm_affine_bwd(x.raw(), G->value.raw(), n->tape[0]->data<float>(), n->tape[1]->data<float>(), gy.raw(),
+                                          want_dx && !first_dx ? gx->raw() : nullptr, want_dx ? gx->raw() : scratch.raw(),
+                                          gg ? gg->data<float>() : nullptr, gb ? gb->data<float>() : nullptr, add_columns ? 1 : 0, ws, wsb,
+                                          rh.rows, rh.hidden, agb_dtype(x), st),
+                 "layernorm backward");
+}
+
 [[noreturn]] void not_on_path(const char* what, const char* name) {
     throw std::runtime_error(std::string(what) + " for op '" + name + "' is not part of the RMSNorm path of this library");
 }
@@ -110,6 +162,10 @@ void vjp_Mul(Node* n, const Tensor& gy) {
 // autodiff_vjp_ops.cpp:351-365; X.grad += dx fused through dx_add == dx == X.grad
 void vjp_LayerNorm(Node* n, const Tensor& gy) {
     StreamGuard g(rule_stream(n));
+    if (n->inputs.size() > 1) {
+        layernorm_affine_backward(n, gy, rule_stream(n));
+        return;
+    }
     Node* X = n->inputs[0].get();
     if (!X->requires_grad()) return;
     const auto rh = rows_hidden(X->value);
@@ -205,6 +261,56 @@ void vjp_LogSumExpRow(Node* n, const Tensor& gy) {
                  "vjp_LogSumExpRow");
 }
 
+// dh = g w, dw = g' h with the logits computed again; dw accumulates in place, a second contribution to h goes through a buffer.
+void vjp_CeWithLogits(Node* n, const Tensor& gy) {
+    if (n->inputs.size() < 3) not_on_path("VJP", "CeWithLogits");
+    StreamGuard g(rule_stream(n));
+    Node* Hn = n->inputs[0].get();
+    Node* Wn = n->inputs[1].get();
+    const Tensor &h = Hn->value, &w = Wn->value, &target = n->inputs[2]->value;
+    const bool want_dh = Hn->requires_grad(), want_dw = Wn->requires_grad();
+    if (!want_dh && !want_dw) return;
+    const auto rh = rows_hidden(h);
+    if (gy.numel() != rh.rows || gy.dtype() != Dtype::Float32)
+        throw std::runtime_error("vjp_CeWithLogits: gy must have one fp32 entry per row");
+    if (Hn == Wn) throw std::runtime_error("vjp_CeWithLogits: h and w must be different nodes");
+    const int64_t vocab = w.shape().dims[0];
+    const size_t wsb = agb_linear_ce_workspace_bytes(1, rh.rows, rh.hidden, vocab, agb_dtype(h));
+    void* ws = workspace(wsb, h, rule_stream(n));
+    Tensor dh;
+    {
+        GradLocks locks({want_dh ? Hn : nullptr, want_dw ? Wn : nullptr});
+        bool first_dh = false, first_dw = false;
+        Tensor* gh = want_dh ? &Hn->open_grad(&first_dh) : nullptr;
+        Tensor* gw = want_dw ? &Wn->open_grad(&first_dw) : nullptr;
+        if (want_dh && !first_dh) dh = Tensor(h.shape(), ag::options(h).with_req_grad(false));
+        check_status(agb_linear_ce_bwd(h.raw(), w.raw(), target.raw(), agb_index(target, "vjp_CeWithLogits"), n->tape[0]->data<float>(),
+                                       gy.data<float>(), want_dh ? (first_dh ? gh->raw() : dh.raw()) : nullptr, want_dw ? gw->raw() : nullptr,
+                                       want_dw && !first_dw ? 1 : 0, rh.rows, rh.hidden, vocab, agb_dtype(h), ws, wsb, rule_stream(n)),
+                     "vjp_CeWithLogits");
+    }
+    if (dh.defined()) Hn->accumulate_grad(dh);
+}
+
+// dz = gy * t * (softmax(z / t) - the teacher's shares), added in place.
+void vjp_KLDivergence(Node* n, const Tensor& gy) {
+    if (n->inputs.size() < 3) not_on_path("VJP", "KLDivergence");
+    StreamGuard g(rule_stream(n));
+    Node* Z = n->inputs[0].get();
+    if (!Z->requires_grad()) return;
+    const Tensor &idx = n->inputs[1]->value, &teacher = n->inputs[2]->value;
+    const auto rh = rows_hidden(Z->value);
+    if (gy.numel() != rh.rows || gy.dtype() != Dtype::Float32)
+        throw std::runtime_error("vjp_KLDivergence: gy must have one fp32 entry per row");
+    std::lock_guard<std::mutex> lock(Z->grad_mutex);
+    bool first = false;
+    Tensor& G = Z->open_grad(&first);
+    check_status(agb_distill_topk_bwd(Z->value.raw(), idx.raw(), agb_index(idx, "vjp_KLDivergence"), teacher.raw(), agb_dtype(teacher),
+                                      n->tape[0]->data<float>(), gy.data<float>(), first ? nullptr : G.raw(), G.raw(), rh.rows, rh.hidden,
+                                      idx.numel() / rh.rows, n->eps, agb_dtype(Z->value), rule_stream(n)),
+                 "vjp_KLDivergence");
+}
+
 #define AG_NOT_ON_PATH(name) \
     void vjp_##name(Node*, const Tensor&) { not_on_path("VJP", #name); }
 AG_NOT_ON_PATH(Sub) AG_NOT_ON_PATH(Div) AG_NOT_ON_PATH(Exp) AG_NOT_ON_PATH(Log) AG_NOT_ON_PATH(Sqrt)
@@ -215,7 +321,7 @@ AG_NOT_ON_PATH(Relu) AG_NOT_ON_PATH(Sigmoid) AG_NOT_ON_PATH(Tanh) AG_NOT_ON_PATH
 AG_NOT_ON_PATH(SiLU) AG_NOT_ON_PATH(Mish) AG_NOT_ON_PATH(LeakyRelu) AG_NOT_ON_PATH(Gaus) AG_NOT_ON_PATH(Parcon)
 AG_NOT_ON_PATH(LiSHT) AG_NOT_ON_PATH(MatMul)
 AG_NOT_ON_PATH(Transpose) AG_NOT_ON_PATH(Linear) AG_NOT_ON_PATH(FMA) AG_NOT_ON_PATH(Dyntanh)
-AG_NOT_ON_PATH(Attention) AG_NOT_ON_PATH(SWIGLU) AG_NOT_ON_PATH(CeWithLogits) AG_NOT_ON_PATH(KLDivergence)
+AG_NOT_ON_PATH(Attention) AG_NOT_ON_PATH(SWIGLU)
 AG_NOT_ON_PATH(MSELoss) AG_NOT_ON_PATH(MAELoss)
 #undef AG_NOT_ON_PATH
 

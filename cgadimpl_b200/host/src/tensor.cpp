@@ -219,6 +219,8 @@ void upload(Tensor& t, const std::vector<float>& host) {
         auto* o = reinterpret_cast<uint16_t*>(staged.data());
         for (int64_t i = 0; i < n; ++i) o[i] = f32_to_bf16(host[i]);
         src = staged.data();
+    } else if (t.dtype() == Dtype::Int32 || t.dtype() == Dtype::Int64) {
+        throw std::invalid_argument("index tensors are made from integers (from_host)");
     } else if (t.dtype() == Dtype::Float64) {
         staged.resize(static_cast<size_t>(n) * 8);
         auto* o = reinterpret_cast<double*>(staged.data());
@@ -268,6 +270,15 @@ Tensor Tensor::rand(const Shape& s, const TensorOptions& o) {
     }
     upload(t, h);
     return t;
+}
+Tensor Tensor::from_host(const int64_t* data, const Shape& s, const TensorOptions& o) {
+    if (o.dtype != Dtype::Int32 && o.dtype != Dtype::Int64) throw std::invalid_argument("from_host: indices need Dtype::Int32 or Dtype::Int64");
+    Tensor t(s, o.with_device(Device::CPU));
+    for (int64_t i = 0; i < t.numel(); ++i) {
+        if (o.dtype == Dtype::Int64) t.data<int64_t>()[i] = data[i];
+        else t.data<int32_t>()[i] = static_cast<int32_t>(data[i]);
+    }
+    return t.to(o.device);
 }
 Tensor Tensor::from_host(const float* data, const Shape& s, const TensorOptions& o) {
     Tensor t(s, o);
@@ -327,6 +338,8 @@ std::vector<float> Tensor::to_vector() const {
     for (int64_t i = 0; i < numel_; ++i) {
         if (dtype() == Dtype::Float32) out[i] = h.data<float>()[i];
         else if (dtype() == Dtype::Bfloat16) out[i] = bf16_to_f32(h.data<uint16_t>()[i]);
+        else if (dtype() == Dtype::Int32) out[i] = static_cast<float>(h.data<int32_t>()[i]);
+        else if (dtype() == Dtype::Int64) out[i] = static_cast<float>(h.data<int64_t>()[i]);
         else out[i] = static_cast<float>(h.data<double>()[i]);
     }
     return out;

@@ -333,3 +333,19 @@ def test_refusals_need_no_device():
     assert bwd(one, one, one, 1, one, one, None, None, 0, 4, 8, 8, 0, one, big, None) == 1
     assert bwd(one, one, one, 1, None, one, one, one, 0, 4, 8, 8, 0, one, big, None) == 1
     assert fwd(None, None, None, 1, None, None, 0, 8, 8, 0, None, 0, None) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,hidden,vocab", [(10, 1835, 2235), (190, 1973, 1818), (2, 4096, 300), (129, 2048, 513), (1, 8192, 255), (64, 1024, 64),
+                                               (250, 4100, 1000)])
+def test_few_tiles_and_a_long_sum(ops, rows, hidden, vocab, dtype):
+    """Sizes whose logits are cut along the hidden axis; rows that take no part among them, and none at all."""
+    h, w, target, gy = make(rows, hidden, vocab, dtype, seed=hidden, ignored=0.3)
+    run_case(ops, h, w, target, gy)
+    run_case(ops, h, w, torch.full_like(target, -1), gy)
+    loss, lse = ops.linear_ce_fwd(h, w, target)
+    n = _lib.lib().agb_linear_ce_workspace_bytes(1, rows, hidden, vocab, ops._dt(h))
+    ws = torch.full((n // 4 + 1,), float("nan"), device="cuda")
+    one, two = ops.linear_ce_bwd(h, w, target, lse, gy, workspace=ws), ops.linear_ce_bwd(h, w, target, lse, gy)
+    assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
