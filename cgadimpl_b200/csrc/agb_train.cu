@@ -228,7 +228,8 @@ int lna_bwd(const agb::LnaBwdArgs& a, float* dgamma, float* dbeta, int accumulat
 int check_kd(int64_t rows, int64_t vocab, int64_t k, float tau, int dtype, int idx_type, int teacher_dtype) {
     if (rows < 0 || vocab <= 0 || k <= 0)
         return fail(AGB_ERR_INVALID_ARG, "rows=%lld vocab=%lld k=%lld", (long long)rows, (long long)vocab, (long long)k);
-    if (!(tau > 0.f) || !(tau < INFINITY)) return fail(AGB_ERR_INVALID_ARG, "temperature %g must be positive and finite", (double)tau);
+    if (!(tau > 0.f) || !(tau < INFINITY) || !(1.f / tau < INFINITY))
+        return fail(AGB_ERR_INVALID_ARG, "temperature %g must be positive and finite, and its reciprocal too", (double)tau);
     if (dtype != AGB_F32 && dtype != AGB_BF16) return fail(AGB_ERR_UNSUPPORTED, "dtype %d (only AGB_F32, AGB_BF16)", dtype);
     if (teacher_dtype != AGB_F32 && teacher_dtype != AGB_BF16)
         return fail(AGB_ERR_UNSUPPORTED, "teacher_dtype %d (only AGB_F32, AGB_BF16)", teacher_dtype);
@@ -441,8 +442,9 @@ int check_ce(int64_t rows, int64_t hidden, int64_t vocab, int dtype, int target_
         return fail(AGB_ERR_INVALID_ARG, "rows=%lld hidden=%lld vocab=%lld", (long long)rows, (long long)hidden, (long long)vocab);
     if (dtype != AGB_F32 && dtype != AGB_BF16) return fail(AGB_ERR_UNSUPPORTED, "dtype %d (only AGB_F32, AGB_BF16)", dtype);
     if (target_type != AGB_I32 && target_type != AGB_I64) return fail(AGB_ERR_INVALID_ARG, "target_type %d (AGB_I32 or AGB_I64)", target_type);
-    if (rows > (1LL << 24) || hidden > (1LL << 20) || vocab > (1LL << 24))
-        return fail(AGB_ERR_UNSUPPORTED, "rows=%lld hidden=%lld vocab=%lld (at most 2^24, 2^20, 2^24)", (long long)rows, (long long)hidden,
+    // rows: the blocks that lay h out count the targets before their own, which grows with the square (13 ms at 2^20 rows)
+    if (rows > (1LL << 20) || hidden > (1LL << 20) || vocab > (1LL << 24))
+        return fail(AGB_ERR_UNSUPPORTED, "rows=%lld hidden=%lld vocab=%lld (at most 2^20, 2^20, 2^24)", (long long)rows, (long long)hidden,
                     (long long)vocab);
     return AGB_OK;
 }
@@ -680,6 +682,8 @@ int agb_linear_ce_bwd(const void* h, const void* w, const void* target, int targ
     AGB_TRY(check_ce(rows, hidden, vocab, dtype, target_type));
     const int elem = dtype == AGB_F32 ? 4 : 2;
     if (!dh && !dw) return fail(AGB_ERR_INVALID_ARG, "neither dh nor dw is asked for");
+    if (dw && dw == w) return fail(AGB_ERR_INVALID_ARG, "dw must not be w: w is read while dw is written");
+    if (dh && (dh == w || dh == dw)) return fail(AGB_ERR_INVALID_ARG, "dh must not be w or dw");
     AGB_TRY(check_ptr(dw, "dw", elem, false));
     if (rows == 0) {
         if (dw && !accumulate_dw)

@@ -186,7 +186,6 @@ __global__ void __launch_bounds__(MAXT) lna_fwd_ring(const LnaFwdArgs a, const L
     }
     __syncthreads();
     pdl_wait();
-    pdl_trigger();
     auto issue = [&](int64_t k, int s) {
         const int64_t r0 = k * g.rows_per_tile;
         const int rows = static_cast<int>(a.rows - r0 < g.rows_per_tile ? a.rows - r0 : g.rows_per_tile);
@@ -277,6 +276,7 @@ __global__ void __launch_bounds__(MAXT) lna_fwd_ring(const LnaFwdArgs a, const L
             phase ^= 1;
         }
     }
+    pdl_trigger();                                     // at the end: 1 to 7 % ahead of triggering at the start
     if (!ok && tid == 0) atomicExch(status, 6 /* AGB_ERR_TIMEOUT */);
 }
 
@@ -370,7 +370,6 @@ __global__ void __launch_bounds__(MAXT) lna_bwd_ring(const LnaBwdArgs a, const L
     }
     __syncthreads();
     pdl_wait();
-    pdl_trigger();
     auto issue = [&](int64_t k, int s) {
         const int64_t r0 = k * g.rows_per_tile;
         const int rows = static_cast<int>(a.rows - r0 < g.rows_per_tile ? a.rows - r0 : g.rows_per_tile);
@@ -502,6 +501,7 @@ __global__ void __launch_bounds__(MAXT) lna_bwd_ring(const LnaBwdArgs a, const L
             phase ^= 1;
         }
     }
+    pdl_trigger();                                     // at the end: 1 to 7 % ahead of triggering at the start
     if (!ok && tid == 0) atomicExch(status, 6 /* AGB_ERR_TIMEOUT */);
     if (!partial) return;
     // ---- the CTA's partial row: rows of a warp first, then warps of the same columns in order

@@ -254,7 +254,8 @@ int agb_layernorm_jvp(const void* y, const void* t, const float* var, void* ty, 
  *   v  = gy * gamma;  dx = rstd * (v - mean_j v - xh * mean_j(v * xh))   [+ dx_add]
  *   dgamma[j] = sum_r gy * xh;  dbeta[j] = sum_r gy           (either may be NULL; added to the old contents with
  *                                                              `accumulate`; rows == 0 gives zeros, or leaves them)
- * dx_add may alias gy or dx.  Sums in fp32, over the CTAs in fp64 in a fixed order: the same call gives the same bits.
+ * dx_add may alias gy or dx; dx may alias x or gy, y may alias x.  Sums in fp32, over the CTAs in fp64 in a fixed order:
+ * the same call gives the same bits.
  * The workspace is only needed for dgamma or dbeta. */
 int agb_layernorm_affine_fwd(const void* x, const void* gamma, const void* beta, void* y, float* mean, float* rstd,
                              int64_t rows, int64_t hidden, float eps, int dtype, agb_stream_t stream);
@@ -273,7 +274,8 @@ int agb_layernorm_affine_bwd(const void* x, const void* gamma, const float* mean
  * holds reaches nothing.  loss, lse, gy: fp32 [rows].  dh or dw may be NULL.
  * AGB_BF16: products of bf16 on the tensor cores with fp32 sums; g is rounded to bf16 as the operand of the two gradient
  * products, dh and dw are rounded once.  AGB_F32: every operand as three bf16 planes and six products, fp32 accuracy.
- * w is read by TMA: aligned to 16 bytes where hidden is a multiple of 8 (AGB_BF16).  Nothing is accumulated atomically: the same
+ * At most 2^20 rows a call.  dh may alias h; dw must not be w.  w is read by TMA: aligned to 16 bytes where hidden is a
+ * multiple of 8 (AGB_BF16).  Nothing is accumulated atomically: the same
  * call gives the same bits.  The workspace (at most about 0.5 GB for w, 0.25 GB for g, plus the rows) need not be kept between the
  * forward and the backward; agb_linear_ce_workspace_bytes needs a device (0 without one). */
 size_t agb_linear_ce_workspace_bytes(int backward, int64_t rows, int64_t hidden, int64_t vocab, int dtype);
@@ -293,8 +295,8 @@ int agb_linear_ce_bwd(const void* h, const void* w, const void* target, int targ
  * An entry whose index lies outside [0, vocab) or whose teacher logit is -inf takes no part; a column named twice gets
  * both shares.  A row without entries has no loss and no gradient, whatever its logits hold: loss = lse = 0, dz = 0
  * (or dz_add).  loss, lse, gy: fp32 [rows].  dz may alias z, dz_add may alias dz.
- * _fwd writes loss and lse, _bwd reads lse, _fwd_bwd does both for callers that know gy beforehand (a sum or a mean) and
- * reads the logits from memory once. */
+ * _fwd writes loss and lse, _bwd reads lse, _fwd_bwd does both in one launch for callers that know gy beforehand (a sum or
+ * a mean); its second look at a row mostly finds it in L2. */
 int agb_distill_topk_fwd(const void* z, const void* idx, int idx_type, const void* teacher, int teacher_dtype,
                          float* loss, float* lse, int64_t rows, int64_t vocab, int64_t k, float temperature,
                          int dtype, agb_stream_t stream);

@@ -287,7 +287,7 @@ def test_refusals_need_no_device():
     assert fwd(one, one, 7, one, 0, one, one, 4, 8, 2, 1.0, 0, None) == 1
     assert fwd(one, one, 1, one, 2, one, one, 4, 8, 2, 1.0, 0, None) == 2
     assert fwd(one, one, 1, one, 0, one, one, 4, 8, 2, 1.0, 2, None) == 2
-    for t in (0.0, -2.0, math.inf, math.nan):
+    for t in (0.0, -2.0, math.inf, math.nan, 1e-40):
         assert fwd(one, one, 1, one, 0, one, one, 4, 8, 2, t, 0, None) == 1
     assert fwd(None, one, 1, one, 0, one, one, 4, 8, 2, 1.0, 0, None) == 1
     assert fwd(one, C.c_void_p(0x1004), 1, one, 0, one, one, 4, 8, 2, 1.0, 0, None) == 3

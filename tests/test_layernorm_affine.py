@@ -294,3 +294,31 @@ def test_refusals_need_no_device():
     assert bwd(one, one, one, one, None, None, one, one, one, 0, one, need, 4, 8, 0, None) == 1
     assert bwd(one, one, one, one, one, odd, one, one, one, 0, one, need, 4, 8, 0, None) == 3
     assert lib.agb_layernorm_affine_bwd_workspace_bytes(4, 0, 0) == 0
+
+
+def test_ring_kernels_do_not_spill():
+    """The 16-byte forms of the one-pass kernels: their loops hold the column sums in registers."""
+    seen = 0
+    for name, r in build.kernel_resources().items():
+        if "lna_bwd_ringI13__nv_bfloat16Li16E" in name or "lna_fwd_ringI13__nv_bfloat16Li16E" in name:
+            seen += 1
+            assert r["spill_stores"] == 0 and r["registers"] <= 128, f"{name}: {r}"
+    assert seen == 6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hidden", [64, 1001, 4096])
+def test_in_place(ops, hidden, dtype):
+    """y over x, dx over gy and dx over x: every element is read before its own place is written."""
+    x, gy, _, gamma, b = make(1500, hidden, dtype, seed=21)
+    y, mean, rstd = ops.layernorm_affine_fwd(x, gamma, b)
+    dx, dg, db = ops.layernorm_affine_bwd(x, gamma, mean, rstd, gy)
+    over = x.clone()
+    assert torch.equal(ops.layernorm_affine_fwd(over, gamma, b, out=over)[0], y)
+    over = gy.clone()
+    got = ops.layernorm_affine_bwd(x, gamma, mean, rstd, over, dx=over)
+    assert torch.equal(got[0], dx) and torch.equal(got[1], dg) and torch.equal(got[2], db)
+    over = x.clone()
+    got = ops.layernorm_affine_bwd(over, gamma, mean, rstd, gy, dx=over)
+    assert torch.equal(got[0], dx) and torch.equal(got[1], dg) and torch.equal(got[2], db)

@@ -325,13 +325,17 @@ def test_refusals_need_no_device():
     assert fwd(one, one, one, 1, one, one, 4, 8, 8, 2, one, big, None) == 2
     assert fwd(one, one, one, 5, one, one, 4, 8, 8, 0, one, big, None) == 1
     assert fwd(one, one, one, 1, one, one, 4, 8, 1 << 25, 0, one, big, None) == 2
+    assert fwd(one, one, one, 1, one, one, (1 << 20) + 1, 8, 8, 0, one, big, None) == 2
     assert fwd(None, one, one, 1, one, one, 4, 8, 8, 0, one, big, None) == 1
     assert fwd(one, one, C.c_void_p(0x1004), 1, one, one, 4, 8, 8, 0, one, big, None) == 3
     assert fwd(one, one, one, 1, None, one, 4, 8, 8, 0, one, big, None) == 1
     assert fwd(one, C.c_void_p(0x1002), one, 1, one, one, 4, 8, 8, 1, one, big, None) == 3
     assert fwd(one, one, one, 1, one, one, 4, 8, 8, 0, None, big, None) == 5
     assert bwd(one, one, one, 1, one, one, None, None, 0, 4, 8, 8, 0, one, big, None) == 1
-    assert bwd(one, one, one, 1, None, one, one, one, 0, 4, 8, 8, 0, one, big, None) == 1
+    two, three = C.c_void_p(0x2000), C.c_void_p(0x3000)
+    assert bwd(one, two, one, 1, None, one, one, three, 0, 4, 8, 8, 0, one, big, None) == 1
+    assert bwd(one, two, one, 1, one, one, one, two, 0, 4, 8, 8, 0, one, big, None) == 1 and b"dw" in lib.agb_last_error()
+    assert bwd(one, two, one, 1, one, one, two, three, 0, 4, 8, 8, 0, one, big, None) == 1
     assert fwd(None, None, None, 1, None, None, 0, 8, 8, 0, None, 0, None) == 0
 
 
@@ -349,3 +353,35 @@ def test_few_tiles_and_a_long_sum(ops, rows, hidden, vocab, dtype):
     ws = torch.full((n // 4 + 1,), float("nan"), device="cuda")
     one, two = ops.linear_ce_bwd(h, w, target, lse, gy, workspace=ws), ops.linear_ce_bwd(h, w, target, lse, gy)
     assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_dh_in_place_of_h(ops, dtype):
+    h, w, target, gy = make(150, 72, 900, dtype, seed=14, ignored=0.2)
+    _, lse = ops.linear_ce_fwd(h, w, target)
+    dh, dw = ops.linear_ce_bwd(h, w, target, lse, gy)
+    over = h.clone()
+    got = ops.linear_ce_bwd(over, w, target, lse, gy, dh=over)
+    assert torch.equal(got[0], dh) and torch.equal(got[1], dw)
+    with pytest.raises(_lib.AgbError):
+        ops.linear_ce_bwd(h, w, target, lse, gy, dw=w)
+
+
+@pytest.mark.gpu
+def test_many_rows_of_a_small_head(ops):
+    """More rows than the blocks that lay them out take 8 of each, most of them without a target."""
+    h, w, target, gy = make(70000, 16, 40, torch.bfloat16, seed=15, ignored=0.9)
+    run_case(ops, h, w, target, gy)
+
+
+def test_matrix_kernels_do_not_spill():
+    """What ptxas made of the matrix kernels: phases 0 to 2 without spills, the epilogue of split fp32 gradients with a few bytes."""
+    seen = 0
+    for name, r in build.kernel_resources().items():
+        if "ce_gemm_kernel" not in name:
+            continue
+        seen += 1
+        limit = 64 if "ELi3EE" in name else 0
+        assert r["spill_stores"] <= limit and r["registers"] <= 168, f"{name}: {r}"
+    assert seen == 8
