@@ -108,13 +108,14 @@ struct LnaPlan {
     int G, block, grid, smem;
     agb::LnaRing ring;
 };
-// Columns a thread takes: one unit where a row has no more than a warp's worth of them; eight where rows are few and a row's latency
+// Columns a thread takes: one unit where a row has no more than a warp's worth of them; eight where a warp then has the row, where rows are few and a row's latency
 // counts (the threads of a row then add up to 1024), and in the backward of rows that are taken element by element, whose instructions and
 // not the sums' registers are the limit (8192 x 2047 fp32: 47 us with eight, 64 us with 32; 4099 x 1001 bf16: 18 and 34 us); else 32, which
 // spreads the fixed cost of a row over more columns (32768 x 4096 bf16: 149 us with 32, 281 us with eight).
 enum LnaWidth { kLnaUnit = 0, kLnaEight = 1, kLnaWide = 2 };
 LnaWidth lna_width(int64_t rows, int64_t units, int n, bool backward, int sms) {
     if (units <= 32) return kLnaUnit;
+    if (units * n <= 256) return kLnaEight;
     return units * n <= 8192 && (rows <= 2LL * sms || (backward && n == 1)) ? kLnaEight : kLnaWide;
 }
 
@@ -395,7 +396,9 @@ CePlan plan_ce(bool backward, int64_t rows, int64_t hidden, int64_t vocab, int d
     // dh: few tiles with a long sum are cut along it, until the GPU has two per SM or a part has 16 slabs
     const int64_t tiles = p.rows_pad / agb::kTM * ceil_div(hidden, agb::kTN), blocks = ceil_div(p.piece, agb::kTK);
     int64_t s = ceil_div(2 * sms, tiles);
-    if (s > blocks / 16) s = blocks / 16;
+    const int64_t slabs = blocks * (p.planes == 3 ? 6 : 1);
+    if (s > slabs / 16) s = slabs / 16;
+    if (s > blocks) s = blocks;
     if (s < 1) s = 1;
     p.k_per_split = static_cast<int>(ceil_div(blocks, s) * agb::kTK);
     p.splits = static_cast<int>(ceil_div(p.piece, p.k_per_split));
@@ -487,14 +490,14 @@ int ce_rows(const CeCall& c, const float* lse, const float* gy, float* loss, flo
     }
     a.loss = loss;
     a.lse_out = lse_out;
-    // a warp per row while the blocks, which all count the targets before their own, stay about a thousand
-    a.per_block = c.rows <= 8192 ? 8 : c.rows <= 16384 ? 16 : agb::kRowsBlock;
+    // a block per row, then a warp per row, while the blocks, which all count the targets before their own, stay about a thousand
+    a.per_block = c.rows <= 8LL * c.d.sms ? 1 : c.rows <= 8192 ? 8 : c.rows <= 16384 ? 16 : agb::kRowsBlock;
     const dim3 grid(static_cast<unsigned>(ceil_div(c.rows, a.per_block)) + agb::kRowsEnd);
     return launch("linear_ce_rows", c.dtype == AGB_F32 ? agb::ce_rows_kernel<float> : agb::ce_rows_kernel<bf16>, grid, dim3(256), 0, c.st, 1, a);
 }
 int ce_pack(const CeCall& c, int64_t col0, int64_t n) {
     if (c.p.direct_w) return AGB_OK;
-    const bool wide = c.hidden >= 256;
+    const bool wide = c.hidden >= 256 && n >= 8LL * c.d.sms;
     int64_t grid = wide ? ceil_div(n, 8) : ceil_div(n * (c.p.k_stride / 2), 256 * 8);
     if (grid > 16LL * c.d.sms) grid = 16LL * c.d.sms;
     auto pack = [&](auto kernel, auto* typed) {
@@ -507,7 +510,7 @@ int ce_pack(const CeCall& c, int64_t col0, int64_t n) {
     return pack(wide ? agb::ce_pack_kernel<bf16, true> : agb::ce_pack_kernel<bf16, false>, static_cast<const bf16*>(nullptr));
 }
 int ce_unpack(const CeCall& c, void* dw, int64_t col0, int64_t n, bool f32, int add) {
-    const bool wide = c.hidden >= 256;
+    const bool wide = c.hidden >= 256 && n >= 8LL * c.d.sms;
     int64_t grid = wide ? ceil_div(n, 8) : ceil_div(n * c.hidden, 256 * 8);
     if (grid > 16LL * c.d.sms) grid = 16LL * c.d.sms;
     auto unpack = [&](auto kernel, auto* from, auto* to) {
@@ -638,7 +641,7 @@ int agb_linear_ce_fwd(const void* h, const void* w, const void* target, int targ
         AGB_TRY(ce_parts(c));
         auto join = [&](auto kernel, auto* typed) {
             typedef decltype(typed) P;
-            return launch("linear_ce_join_parts", kernel, dim3(static_cast<unsigned>(rows)), dim3(256), 0, c.st, 1, c.at<float>(c.p.z), c.p.z_splits,
+            return launch("linear_ce_join_parts", kernel, dim3(static_cast<unsigned>(rows)), dim3(vocab <= 2048 ? 256 : 1024), 0, c.st, 1, c.at<float>(c.p.z), c.p.z_splits,
                           c.p.rows_pad, c.p.piece, static_cast<int>(vocab), c.at<int>(c.p.count), c.at<int>(c.p.target_of), c.at<int>(c.p.row_of),
                           static_cast<P>(h), static_cast<P>(w), static_cast<int>(hidden), loss, lse);
         };

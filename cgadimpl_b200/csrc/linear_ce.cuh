@@ -180,37 +180,38 @@ __device__ __forceinline__ int ce_target(const CeRowsArgs& a, int64_t r) {
 
 // One row into its planes; `vec`: 16-byte loads are possible.  Loads are issued in batches before the stores that may alias them.
 template <typename T>
-__device__ __forceinline__ void ce_copy_row(const T* src, __nv_bfloat16* dst, int cols, int64_t stride, int64_t plane, bool vec, int lane) {
+__device__ __forceinline__ void ce_copy_row(const T* src, __nv_bfloat16* dst, int cols, int64_t stride, int64_t plane, bool vec, int lane,
+                                            int lanes) {
     constexpr int B = 8;
     if (sizeof(T) == 2 && vec) {
         const uint4* s = reinterpret_cast<const uint4*>(src);
         uint4* d = reinterpret_cast<uint4*>(dst);
         const int n = cols / 8;
-        for (int i0 = lane; i0 < n; i0 += 32 * B) {
+        for (int i0 = lane; i0 < n; i0 += lanes * B) {
             uint4 v[B];
 #pragma unroll
             for (int b = 0; b < B; ++b)
-                if (i0 + 32 * b < n) v[b] = s[i0 + 32 * b];
+                if (i0 + lanes * b < n) v[b] = s[i0 + lanes * b];
 #pragma unroll
             for (int b = 0; b < B; ++b)
-                if (i0 + 32 * b < n) d[i0 + 32 * b] = v[b];
+                if (i0 + lanes * b < n) d[i0 + lanes * b] = v[b];
         }
         return;
     }
     uint32_t* d = reinterpret_cast<uint32_t*>(dst);    // two columns at a time: the stride is a multiple of 8
     const int n = static_cast<int>(stride / 2);
     const int64_t p32 = plane / 2;
-    for (int i0 = lane; i0 < n; i0 += 32 * B) {
+    for (int i0 = lane; i0 < n; i0 += lanes * B) {
         T v[B][2];
 #pragma unroll
         for (int b = 0; b < B; ++b) {
-            const int c = 2 * (i0 + 32 * b);
+            const int c = 2 * (i0 + lanes * b);
             v[b][0] = c < cols ? src[c] : T(0.f);
             v[b][1] = c + 1 < cols ? src[c + 1] : T(0.f);
         }
 #pragma unroll
         for (int b = 0; b < B; ++b) {
-            const int i = i0 + 32 * b;
+            const int i = i0 + lanes * b;
             if (i >= n) continue;
             if (sizeof(T) == 2) {
                 d[i] = (__float_as_uint(Vec<T>::load1(&v[b][0])) >> 16) | (__float_as_uint(Vec<T>::load1(&v[b][1])) & 0xffff0000u);
@@ -293,9 +294,12 @@ __global__ void __launch_bounds__(256) ce_rows_kernel(const CeRowsArgs a) {
     }
     __syncthreads();
     const bool vec = sizeof(T) == 2 && a.cols % 8 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
-    for (int i = warp; i < a.per_block; i += 8)
+    // a warp per row, or the block where it has one row only
+    const bool alone = a.per_block == 1;
+    for (int i = alone ? 0 : warp; i < a.per_block; i += 8)
         if (where[i] >= 0)
-            ce_copy_row(static_cast<const T*>(a.x) + (r0 + i) * a.cols, a.dst + where[i] * a.stride, a.cols, a.stride, plane, vec, lane);
+            ce_copy_row(static_cast<const T*>(a.x) + (r0 + i) * a.cols, a.dst + where[i] * a.stride, a.cols, a.stride, plane, vec,
+                        alone ? threadIdx.x : lane, alone ? 256 : 32);
 }
 
 // Rows [row0, row0 + rows) of w into dst [planes][rows_pad][stride]: what W needs where TMA cannot read it as it is.  LONG: a warp per row.
@@ -307,7 +311,7 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const T* w, int64_t rows, 
     if constexpr (LONG) {
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
         for (int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + warp; r < rows; r += static_cast<int64_t>(gridDim.x) * 8)
-            ce_copy_row(w + r * cols, dst + r * stride, cols, stride, rows_pad * stride, false, lane);
+            ce_copy_row(w + r * cols, dst + r * stride, cols, stride, rows_pad * stride, false, lane, 32);
         return;
     }
     constexpr int B = 8;
@@ -797,10 +801,10 @@ __global__ void __launch_bounds__(256) ce_join_kernel(const float2* pairs, int n
 // Few tiles and a long sum: the logits as fp32 parts [splits][rows_pad][stride] of K, each part a CTA's.  This is the join for them: a block
 // per row adds the parts, takes the maximum and the sum, and goes on as ce_join_kernel does.
 template <typename T>
-__global__ void __launch_bounds__(256) ce_join_parts_kernel(const float* parts, int splits, int64_t rows_pad, int64_t stride, int vocab,
+__global__ void __launch_bounds__(1024) ce_join_parts_kernel(const float* parts, int splits, int64_t rows_pad, int64_t stride, int vocab,
                                                             const int* count, const int* target_of, const int* row_of, const T* h, const T* w,
                                                             int hidden, float* loss, float* lse) {
-    __shared__ float red[8][3];
+    __shared__ float red[32][3];
     __shared__ float z_there;
     pdl_wait();
     pdl_trigger();
@@ -811,11 +815,10 @@ __global__ void __launch_bounds__(256) ce_join_parts_kernel(const float* parts, 
     const T* hr = h + static_cast<int64_t>(r) * hidden;
     const T* wr = w + static_cast<int64_t>(target) * hidden;
 #pragma unroll 4
-    for (int c = threadIdx.x; c < hidden; c += 256) z = __fmaf_rn(Vec<T>::load1(hr + c), Vec<T>::load1(wr + c), z);
+    for (int c = threadIdx.x; c < hidden; c += blockDim.x) z = __fmaf_rn(Vec<T>::load1(hr + c), Vec<T>::load1(wr + c), z);
     float m = -INFINITY, s = 0.f;
     const float* p = parts + i * stride;
-#pragma unroll 2
-    for (int c = threadIdx.x * 4; c < vocab; c += 1024) {
+    for (int c = threadIdx.x * 4; c < vocab; c += 4 * blockDim.x) {
         float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
         for (int k = 0; k < splits; ++k) {
@@ -845,7 +848,7 @@ __global__ void __launch_bounds__(256) ce_join_parts_kernel(const float* parts, 
     }
     __syncthreads();
     if (threadIdx.x) return;
-    for (int q = 1; q < 8; ++q) {
+    for (int q = 1; q < static_cast<int>(blockDim.x >> 5); ++q) {
         z = __fadd_rn(z, red[q][0]);
         join_pair(m, s, red[q][1], red[q][2]);
     }
