@@ -136,7 +136,7 @@ LnaPlan plan_lna(int64_t rows, int64_t hidden, int elem, bool whole, int64_t uni
     }
     const int slack = whole ? 0 : 32;
     const int64_t tile = ceil_div(per_tile * row_bytes + slack, 128) * 128, sums = arrays == 2 && per_tile > 1 ? 2 * hidden * 4 : 0;
-    int ctas = (limit >= 1024 || upt == 1 ? 1024 : 512) / p.block;          // registers: 64 or 128 a thread
+    int ctas = (limit >= 1024 || upt == 1 ? 1024 : arrays == 1 && !whole && p.block <= 256 ? 768 : 512) / p.block;   // registers: 64, 80 or 128
     if (ctas > kLnaCtas) ctas = kLnaCtas;
     if (ctas < 1) ctas = 1;
     int stages = 0;
@@ -176,6 +176,11 @@ int lna_fwd(const agb::LnaFwdArgs& a, const agb_int::Device& d, cudaStream_t st)
     if (p.ring.stages > 0) {
         if (width == kLnaUnit) return lna_fwd_launch<T, UB, 1, 512>(a, p, d, st);
         if (width == kLnaEight) return lna_fwd_launch<T, UB, 8 / N, 1024>(a, p, d, st);
+        // element by element: blocks of 256 at 80 registers a thread, three per SM instead of two (16384 x 4097 bf16 115 -> 102 us; the 16-byte
+        // form spills there, 16384 x 8192 bf16 105 -> 151 us)
+        if constexpr (UB < 16) {
+            if (p.block <= 256) return lna_fwd_launch<T, UB, 32 / N, 256>(a, p, d, st);
+        }
         return lna_fwd_launch<T, UB, 32 / N, 512>(a, p, d, st);
     }
     agb::lna_fwd_wide<T, UB><<<static_cast<unsigned>(grid_for(a.rows, 1024, 1024, d.sms, 2)), 1024, 0, st>>>(a);
