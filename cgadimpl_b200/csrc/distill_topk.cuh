@@ -6,8 +6,8 @@
 // distributed shared memory), with a running maximum and sum; the backward reads the slice again, from L2, and writes it.  Few rows:
 // eight slices in a cluster, short enough to be loaded into registers before anything else is done and to stay there.  Short rows: a
 // warp each, no block barrier anywhere.  The K columns of the teacher are set again after the slice is written, from unrounded values.
-// Bound by memory: the K columns are a few KB against a row of hundreds.  4096 x 131072 bf16, k = 64: forward 167 us (the copy rate), backward
-// 344 us (97 % of it), both in one call 476 us (70 %): there a row's sum and its gradient follow one another, and a block that joins its
+// Bound by memory: the K columns are a few KB against a row of hundreds.  4096 x 131072 bf16, k = 64: forward 168 us (the copy rate), backward
+// 353 us (94 % of it), both in one call 495 us (67 %): there a row's sum and its gradient follow one another, and a block that joins its
 // sums or gathers the teacher's columns loads nothing.  Tried and slower: a ring of bulk copies that run ahead into the next row (612 us),
 // slices of 32 KB in registers (976 us: the fixed 14000 clocks of a block against 6000 for its slice), L2 eviction hints (no change).
 #pragma once

@@ -1,6 +1,7 @@
 /*
- * agb.h -- C ABI of libagb_cuda.so: the RMSNorm forward / VJP / JVP path of cgadimpl,
- * hand-written for NVIDIA B200 (sm_100a).
+ * agb.h -- C ABI of libagb_cuda.so: the RMSNorm forward / VJP / JVP path of cgadimpl, and the end of a model that trains
+ * beside it (LayerNorm with weight and bias, the vocabulary loss from the hidden states, distillation from a teacher's
+ * largest logits), hand-written for NVIDIA B200 (sm_100a).
  *
  * Style follows cgadimpl's own raw-pointer kernel plugin (`ag::kernels::cuda()` loaded with
  * `load_cuda_plugin("./libagkernels_cuda.so")`, cgadimpl/Tests/test_kernels_gpu.cpp:39-148):
@@ -276,8 +277,8 @@ int agb_layernorm_affine_bwd(const void* x, const void* gamma, const float* mean
  * products, dh and dw are rounded once.  AGB_F32: every operand as three bf16 planes and six products, fp32 accuracy.
  * At most 2^20 rows a call.  dh may alias h; dw must not be w.  w is read by TMA: aligned to 16 bytes where hidden is a
  * multiple of 8 (AGB_BF16).  Nothing is accumulated atomically: the same
- * call gives the same bits.  The workspace (at most about 0.5 GB for w, 0.25 GB for g, plus the rows) need not be kept between the
- * forward and the backward; agb_linear_ce_workspace_bytes needs a device (0 without one). */
+ * call gives the same bits.  The workspace (at most about 0.5 GB for w where TMA cannot read it as it is, 0.25 GB for g, and per row the
+ * operands and, forward, vocab / 16 bytes) need not be kept between the forward and the backward; agb_linear_ce_workspace_bytes needs a device (0 without one). */
 size_t agb_linear_ce_workspace_bytes(int backward, int64_t rows, int64_t hidden, int64_t vocab, int dtype);
 int agb_linear_ce_fwd(const void* h, const void* w, const void* target, int target_type, float* loss, float* lse,
                       int64_t rows, int64_t hidden, int64_t vocab, int dtype, void* workspace, size_t workspace_bytes,
